@@ -1,0 +1,100 @@
+// Loads and stores of eight values between memory of any of the three types and 32-bit registers.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "block_ops.h"
+
+namespace pccl {
+namespace block {
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+// One rounding to nearest even from 32 bits.
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight consecutive values, as they lie in memory: 16 bytes of a 16-bit type, 32 of a 32-bit one.
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+
+template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store_raw8(T* p, const Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+}
+
+__device__ __forceinline__ void unpack2(uint32_t w, float* f, __nv_bfloat16) {
+  f[0] = __uint_as_float(w << 16);
+  f[1] = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float* f, __half) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  f[0] = v.x;
+  f[1] = v.y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T> __device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[4 * i] = __uint_as_float(r.v[i].x);
+      f[4 * i + 1] = __uint_as_float(r.v[i].y);
+      f[4 * i + 2] = __uint_as_float(r.v[i].z);
+      f[4 * i + 3] = __uint_as_float(r.v[i].w);
+    }
+  } else {
+    unpack2(r.v[0].x, f, T());
+    unpack2(r.v[0].y, f + 2, T());
+    unpack2(r.v[0].z, f + 4, T());
+    unpack2(r.v[0].w, f + 6, T());
+  }
+}
+template <typename T> __device__ __forceinline__ Raw8<T> pack8(const float* f) {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      r.v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                          __float_as_uint(f[4 * i + 3]));
+  } else {
+    r.v[0] = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+  }
+  return r;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+}  // namespace block
+}  // namespace pccl
+
+// Calls BODY with the type `T` that stands for a DType.
+#define PCCL_BLOCK_TYPES(DTYPE, T, ...)                                                    \
+  switch (DTYPE) {                                                                         \
+    case ::pccl::block::DType::kF32: { using T = float; __VA_ARGS__; break; }              \
+    case ::pccl::block::DType::kF16: { using T = __half; __VA_ARGS__; break; }             \
+    case ::pccl::block::DType::kBF16: { using T = __nv_bfloat16; __VA_ARGS__; break; }     \
+  }

@@ -10,6 +10,7 @@
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
+#include "block/block_bindings.h"
 #include "common/launch.h"
 #include "common/util.h"
 #include "engine/engine.h"
@@ -302,5 +303,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_static("registerOpt", &Environs::register_option);
 
   bind_fused_ops(m);
+  bind_block_ops(m);
   bind_rdma(m);
 }

@@ -13,9 +13,18 @@ per (local expert, source rank) is reserved so that no token is ever dropped.  W
 process group (one GPU) an ordinary CUDA buffer stands in for the symmetric heap.
 Construction is collective.  The reference has no MoE operator; the workload is its
 all-to-all template's target use (pccl/dsl/algorithms/ring.py, build_alltoall).
+
+For layers that route otherwise, or that are trained, the steps around the experts' products are operators of
+their own, on ordinary tensors of one GPU and with gradients:
+
+``route_topk``   scores (softmax or sigmoid, a bias for balance, groups), top-k, weights, expert order;
+``dispatch``     token rows into expert order, one copy per choice;
+``combine``      the experts' rows back to their tokens, weighted and summed.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -145,3 +154,69 @@ def route(x: torch.Tensor, wg: torch.Tensor):
     counts = torch.empty(experts, dtype=torch.int32, device=x.device)
     native.moe_route(x.contiguous(), wg.contiguous(), scratch, idx, gate, slot, counts)
     return idx, gate, slot, counts
+
+
+class Routing(NamedTuple):
+    """What ``route_topk`` chose.  Rows ``offsets[e]`` to ``offsets[e + 1]`` of a batch in expert order belong to
+    expert ``e``, tokens in order; rows from ``offsets[-1]`` on are unused (there are some only with a mask)."""
+
+    idx: torch.Tensor       # [tokens, top_k] int32, best first; -1 for masked tokens
+    weights: torch.Tensor   # [tokens, top_k] float32, differentiable
+    rows: torch.Tensor      # [tokens, top_k] int32: row of each choice in expert order; -1 for masked tokens
+    offsets: torch.Tensor   # [experts + 1] int32
+
+
+_block = None
+
+
+def _block_native():
+    global _block
+    if _block is None:
+        _block = _engine.load_native().block
+    return _block
+
+
+def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor] = None, scoring: str = "softmax",
+               groups: int = 1, top_groups: Optional[int] = None, group_score: str = "max", renormalise: bool = True,
+               scale: float = 1.0, mask: Optional[torch.Tensor] = None) -> Routing:
+    """Choose ``top_k`` experts per token from router logits ``[tokens, experts]`` (float32, float16, bfloat16).
+
+    ``p = softmax(logits)`` or ``sigmoid(logits)`` (``scoring``).  Experts are ranked by ``s = p + bias`` (``bias``
+    float32 ``[experts]``, for an even load; it changes the choice alone and has no gradient).  With ``groups``
+    equal groups of neighbouring experts only those of the ``top_groups`` best stay, a group counting by its best
+    score (``group_score="max"``) or the sum of its two best (``"top2"``).  Ties go to the lowest number; scores
+    are told apart to 64 bits (without a bias by the logits themselves).  The weights are
+    ``scale * p / sum(p over the choice)``, or ``scale * p`` with ``renormalise=False``.
+
+    A logit of minus infinity or NaN takes an expert out: its score is minus infinity whatever its bias, it is
+    chosen only where nothing else is left, and then with weight 0.  Plus infinity counts as the largest finite
+    logit.  Tokens where ``mask`` (bool ``[tokens]``) is false choose nothing: index and row -1, weight 0.
+
+    Up to 1024 experts, 32 groups and 31 choices.  ``weights`` carries the gradient of ``logits`` (once: it cannot
+    be differentiated twice); the order of the choices within an expert is that of the tokens, on every run.
+    """
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"route_topk: scoring must be 'softmax' or 'sigmoid', not {scoring!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(f"route_topk: group_score must be 'max' or 'top2', not {group_score!r}")
+    return Routing(*_block_native().route_topk(logits, top_k, bias, scoring == "sigmoid", groups,
+                                               groups if top_groups is None else top_groups, group_score == "top2",
+                                               renormalise, scale, mask))
+
+
+def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """``out[routing.rows[t, k]] = x[t]``: ``[tokens * top_k, hidden]`` in expert order, for the experts' products.
+
+    Rows from ``routing.offsets[-1]`` on become zero.  The gradient of ``x`` sums its copies in 32 bits.  ``x`` is
+    float32, float16 or bfloat16 ``[tokens, hidden]``, rows at any distance.
+    """
+    return _block_native().dispatch(x, routing.rows, routing.offsets)
+
+
+def combine(y: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """``out[t] = sum_k routing.weights[t, k] * y[routing.rows[t, k]]``: the experts' rows back to their tokens.
+
+    The sum is taken in 32 bits in the order of the choices and rounded once; a token without choices gets zeros.
+    Gradients go to ``y`` (zero in rows that no choice reads) and to ``routing.weights``.
+    """
+    return _block_native().combine(y, routing.weights, routing.rows, routing.offsets)
