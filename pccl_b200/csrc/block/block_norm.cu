@@ -33,8 +33,12 @@ namespace block {
 
 namespace {
 
-constexpr int kVecs = 2;                       // groups of eight values a thread holds of its row
-constexpr int kHeld = 8 * kVecs;
+constexpr int kHeld = 16;                      // values a thread holds of its row
+
+// They stand in groups of consecutive columns, as many as 16 bytes of the widest type hold: a warp then touches
+// whole 32-byte sectors in every access.  (Eight columns of 32 bits a thread, as two accesses 32 bytes apart from
+// lane to lane, moved every sector twice.)
+template <typename TX, typename TR> constexpr int kGroup = sizeof(TX) == 4 || sizeof(TR) == 4 ? 4 : 8;
 
 struct NormParams {
   NormArgs a;
@@ -49,145 +53,118 @@ struct NormParams {
   int workers;
 };
 
-// Column of value j of group v held by a thread: eight in a row where rows are aligned, else a thread's values
-// stand a whole row of threads apart, so that neighbours read neighbours.
-template <bool kVec> __device__ __forceinline__ int column(int v, int j, int tid, int width) {
-  return kVec ? (v * width + tid) * 8 + j : (v * 8 + j) * width + tid;
+// Column of value j of group v held by a thread: G in a row where rows are aligned, else a thread's values stand a
+// whole row of threads apart, so that neighbours read neighbours.
+template <bool kVec, int G> __device__ __forceinline__ int column(int v, int j, int tid, int width) {
+  return kVec ? (v * width + tid) * G + j : (v * G + j) * width + tid;
 }
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_row(const T* row, int hidden, int tid, int width, float* f) {
+// G values as they lie in memory.
+template <typename T, int G> struct alignas(G * sizeof(T) > 16 ? 16 : G * sizeof(T)) Raw { uint32_t w[G * sizeof(T) / 4]; };
+
+template <typename T, int G> __device__ __forceinline__ void unpack(const Raw<T, G>& r, float2* f) {
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    if constexpr (kVec) {
-      const int at = (v * width + tid) * 8;
-      if (at < hidden) {
-        unpack8<T>(load_raw8<T>(row + at), f + 8 * v);
-      } else {
+  for (int i = 0; i < G / 2; ++i) {
+    if constexpr (sizeof(T) == 4) f[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else unpack2(r.w[i], &f[i].x, T());
+  }
+}
+template <typename T, int G> __device__ __forceinline__ Raw<T, G> pack(const float2* f) {
+  Raw<T, G> r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[8 * v + j] = 0.f;
-      }
+  for (int i = 0; i < G / 2; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r.w[2 * i] = __float_as_uint(f[i].x);
+      r.w[2 * i + 1] = __float_as_uint(f[i].y);
+    } else {
+      r.w[i] = pack2(f[i].x, f[i].y, T());
+    }
+  }
+  return r;
+}
+
+// The values of group v, from the row itself.
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void load_group(const T* row, int v, int hidden, int tid, int width, float2* to) {
+  if constexpr (kVec) {
+    const int at = (v * width + tid) * G;
+    if (at < hidden) {
+      unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(row + at), to);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = column<false>(v, j, tid, width);
-        f[8 * v + j] = at < hidden ? to_f32<T>(row[at]) : 0.f;
-      }
+      for (int j = 0; j < G / 2; ++j) to[j] = make_float2(0.f, 0.f);
+    }
+  } else {
+    float* f = reinterpret_cast<float*>(to);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int at = column<false, G>(v, j, tid, width);
+      f[j] = at < hidden ? to_f32<T>(row[at]) : 0.f;
     }
   }
 }
-template <typename T, bool kVec>
-__device__ __forceinline__ void store_row(T* row, int hidden, int tid, int width, const float* f) {
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void store_group(T* row, int v, int hidden, int tid, int width, const float2* from) {
+  if constexpr (kVec) {
+    const int at = (v * width + tid) * G;
+    if (at < hidden) *reinterpret_cast<Raw<T, G>*>(row + at) = pack<T, G>(from);
+  } else {
+    const float* f = reinterpret_cast<const float*>(from);
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    if constexpr (kVec) {
-      const int at = (v * width + tid) * 8;
-      if (at < hidden) store_raw8<T>(row + at, pack8<T>(f + 8 * v));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = column<false>(v, j, tid, width);
-        if (at < hidden) row[at] = from_f32<T>(f[8 * v + j]);
-      }
+    for (int j = 0; j < G; ++j) {
+      const int at = column<false, G>(v, j, tid, width);
+      if (at < hidden) row[at] = from_f32<T>(f[j]);
     }
   }
+}
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void store_row(T* row, int hidden, int tid, int width, const float2* f) {
+#pragma unroll
+  for (int v = 0; v < kHeld / G; ++v) store_group<T, kVec, G>(row, v, hidden, tid, width, f + v * (G / 2));
 }
 // A weight vector is of the activations' type or of 32 bits.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_weight(const Weight& w, int64_t first, int hidden, int tid, int width, float* f) {
-  if (w.f32) load_row<float, kVec>(static_cast<const float*>(w.ptr) + first, hidden, tid, width, f);
-  else load_row<T, kVec>(static_cast<const T*>(w.ptr) + first, hidden, tid, width, f);
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void load_weight(const Weight& w, int64_t first, int hidden, int tid, int width, float2* f) {
+#pragma unroll
+  for (int v = 0; v < kHeld / G; ++v) {
+    if (w.f32) load_group<float, kVec, G>(static_cast<const float*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
+    else load_group<T, kVec, G>(static_cast<const T*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
+  }
 }
 
 // ---- ring ------------------------------------------------------------------------------------------------
-// A plane holds 16 bytes per thread of a row; an input of T takes kVecs * sizeof(T) / 2 planes.
-template <typename T> constexpr int kPlanes = kVecs * static_cast<int>(sizeof(T)) / 2;
+// A thread's share of a row of T in the ring: kHeld values.
+template <typename T> constexpr int kBytes = kHeld * static_cast<int>(sizeof(T));
 
-__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-               "l"(from) : "memory");
+// `kSize` bytes (8 or 16), or as many zeros.
+template <int kSize> __device__ __forceinline__ void copy_async(void* to, const void* from, bool zeros) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  const int size = zeros ? 0 : kSize;
+  if constexpr (kSize == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(size) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(size) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void fetch_row(uint4* plane, const T* row, int hidden, int tid, int width) {
-  constexpr int kQ = sizeof(T) / 2;
+template <typename T, int G>
+__device__ __forceinline__ void fetch_row(char* slot, const T* row, int hidden, int tid, int width) {
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const int at = (v * width + tid) * 8;
-    if (at < hidden)
-#pragma unroll
-      for (int q = 0; q < kQ; ++q)
-        copy_async(plane + (v * kQ + q) * width + tid, reinterpret_cast<const uint4*>(row + at) + q);
+  for (int v = 0; v < kHeld / G; ++v) {
+    const int at = (v * width + tid) * G;
+    const bool beyond = at >= hidden;
+    copy_async<G * sizeof(T)>(slot + (v * width + tid) * (G * sizeof(T)), row + (beyond ? 0 : at), beyond);
   }
 }
-template <typename T>
-__device__ __forceinline__ void held_row(const uint4* plane, int hidden, int tid, int width, float* f) {
-  constexpr int kQ = sizeof(T) / 2;
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    if ((v * width + tid) * 8 < hidden) {
-      Raw8<T> r;
-#pragma unroll
-      for (int q = 0; q < kQ; ++q) r.v[q] = plane[(v * kQ + q) * width + tid];
-      unpack8<T>(r, f + 8 * v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[8 * v + j] = 0.f;
-    }
-  }
-}
-// The eight values of group v: from a ring plane, or from the row itself.
-template <typename T, bool kVec, bool kHeldRow>
-__device__ __forceinline__ void take8(const uint4* plane, const T* row, int v, int hidden, int tid, int width, float* f) {
-  if constexpr (kHeldRow) {
-    constexpr int kQ = sizeof(T) / 2;
-    Raw8<T> r;
-#pragma unroll
-    for (int q = 0; q < kQ; ++q) r.v[q] = plane[(v * kQ + q) * width + tid];
-    unpack8<T>(r, f);
-    if ((v * width + tid) * 8 >= hidden) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    }
-  } else if constexpr (kVec) {
-    const int at = (v * width + tid) * 8;
-    if (at < hidden) {
-      unpack8<T>(load_raw8<T>(row + at), f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = column<false>(v, j, tid, width);
-      f[j] = at < hidden ? to_f32<T>(row[at]) : 0.f;
-    }
-  }
-}
-template <typename T, bool kVec>
-__device__ __forceinline__ void put8(T* row, int v, int hidden, int tid, int width, const float* f) {
-  if constexpr (kVec) {
-    const int at = (v * width + tid) * 8;
-    if (at < hidden) store_raw8<T>(row + at, pack8<T>(f));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = column<false>(v, j, tid, width);
-      if (at < hidden) row[at] = from_f32<T>(f[j]);
-    }
-  }
-}
-__device__ __forceinline__ void slots_load8(const uint4* plane, int v, int tid, int width, float* f) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 q = reinterpret_cast<const float4*>(plane)[(2 * v + i) * width + tid];
-    f[4 * i] = q.x; f[4 * i + 1] = q.y; f[4 * i + 2] = q.z; f[4 * i + 3] = q.w;
-  }
+
+// The values of group v: from the ring, or from the row itself.
+template <typename T, bool kVec, bool kHeldRow, int G>
+__device__ __forceinline__ void take(const char* slot, const T* row, int v, int hidden, int tid, int width, float2* to) {
+  if constexpr (kHeldRow) unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(slot + (v * width + tid) * (G * sizeof(T))), to);
+  else load_group<T, kVec, G>(row, v, hidden, tid, width, to);
 }
 
 // Sum over the threads of a row; `sums` alternates between two sets so that one barrier a call is enough.  Sets
@@ -213,31 +190,32 @@ __device__ __forceinline__ float row_sum(float v, RowSums& sums, int* turn) {
   return v;
 }
 
-// A thread's slots of one weight: kHeld 32-bit values.
-constexpr int kWeightPlanes = kHeld / 4;
-__device__ __forceinline__ void slots_store(uint4* plane, int tid, int width, const float* f) {
+// A thread's slots of one weight: kHeld 32-bit values, four to an access.
+__device__ __forceinline__ void slots_store(char* slot, int tid, int width, const float2* f) {
 #pragma unroll
-  for (int i = 0; i < kWeightPlanes; ++i) reinterpret_cast<float4*>(plane)[i * width + tid] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  for (int i = 0; i < kHeld / 4; ++i)
+    reinterpret_cast<float4*>(slot)[i * width + tid] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
 }
-__device__ __forceinline__ void slots_load(const uint4* plane, int tid, int width, float* f) {
+template <int G> __device__ __forceinline__ void slots_load(const char* slot, int v, int tid, int width, float2* f) {
 #pragma unroll
-  for (int i = 0; i < kWeightPlanes; ++i) {
-    const float4 q = reinterpret_cast<const float4*>(plane)[i * width + tid];
-    f[4 * i] = q.x; f[4 * i + 1] = q.y; f[4 * i + 2] = q.z; f[4 * i + 3] = q.w;
+  for (int i = 0; i < G / 4; ++i) {
+    const float4 q = reinterpret_cast<const float4*>(slot)[(v * (G / 4) + i) * width + tid];
+    f[2 * i] = make_float2(q.x, q.y);
+    f[2 * i + 1] = make_float2(q.z, q.w);
   }
 }
 
 // g1 = post_gamma * gate of one group of rows into its slots (what is absent counts as 1).
-template <typename T, bool kVec>
-__device__ __forceinline__ void form_g1(const NormArgs& a, int64_t group, uint4* plane, int tid, int width) {
-  float f[kHeld], w[kHeld];
-  if (a.post_gamma.ptr) load_weight<T, kVec>(a.post_gamma, 0, a.hidden, tid, width, f);
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void form_g1(const NormArgs& a, int64_t group, char* slot, int tid, int width) {
+  float2 f[kHeld / 2], w[kHeld / 2];
+  if (a.post_gamma.ptr) load_weight<T, kVec, G>(a.post_gamma, 0, a.hidden, tid, width, f);
   if (a.gate.ptr) {
-    load_weight<T, kVec>(a.gate, group * a.hidden, a.hidden, tid, width, w);
+    load_weight<T, kVec, G>(a.gate, group * a.hidden, a.hidden, tid, width, w);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) f[i] = a.post_gamma.ptr ? f[i] * w[i] : w[i];
+    for (int i = 0; i < kHeld / 2; ++i) f[i] = a.post_gamma.ptr ? mul2(f[i], w[i]) : w[i];
   }
-  slots_store(plane, tid, width, f);
+  slots_store(slot, tid, width, f);
 }
 
 // First row of worker w's run; w = workers gives the number of rows.
@@ -245,26 +223,28 @@ __device__ __forceinline__ int64_t run_start(int64_t rows, int workers, int w) {
   return rows / workers * w + min(static_cast<int64_t>(w), rows % workers);
 }
 
-// Slots of a worker, in planes: gamma, g1, (backward) the sum that becomes dpost_gamma, then the rows of the ring.
+// Slots of a worker, in bytes a thread: gamma, g1, (backward) the sum that becomes dpost_gamma, then the rows of
+// the ring.
 __host__ __device__ __forceinline__ bool has_g1(const NormArgs& a) { return a.post_gamma.ptr || a.gate.ptr; }
-__host__ __device__ __forceinline__ int weight_planes(const NormArgs& a, bool backward) {
-  return kWeightPlanes * ((a.gamma.ptr ? 1 : 0) + (has_g1(a) ? 1 : 0) + (backward && a.post_gamma.ptr && a.gate.ptr ? 1 : 0));
+__host__ __device__ __forceinline__ int weight_bytes(const NormArgs& a, bool backward) {
+  return kBytes<float> * ((a.gamma.ptr ? 1 : 0) + (has_g1(a) ? 1 : 0) + (backward && a.post_gamma.ptr && a.gate.ptr ? 1 : 0));
 }
-template <typename TX, typename TR> __host__ __device__ __forceinline__ int forward_planes(const NormArgs& a) {
-  return kPlanes<TR> + (a.x ? kPlanes<TX> : 0);
+template <typename TX, typename TR> __host__ __device__ __forceinline__ int forward_bytes(const NormArgs& a) {
+  return kBytes<TR> + (a.x ? kBytes<TX> : 0);
 }
-template <typename TX, typename TR> __host__ __device__ __forceinline__ int backward_planes(const NormArgs& a, const NormGrads& g) {
-  int planes = 0;
-  if (g.dh) planes += kPlanes<TR>;
-  if (g.dy) planes += kPlanes<TX> + (g.h ? kPlanes<float> : kPlanes<TR>);
-  if (a.x) planes += kPlanes<TX>;
-  return planes;
+template <typename TX, typename TR> __host__ __device__ __forceinline__ int backward_bytes(const NormArgs& a, const NormGrads& g) {
+  int bytes = 0;
+  if (g.dh) bytes += kBytes<TR>;
+  if (g.dy) bytes += kBytes<TX> + (g.h ? kBytes<float> : kBytes<TR>);
+  if (a.x) bytes += kBytes<TX>;
+  return bytes;
 }
 
 template <typename TX, typename TR, bool kVec, int kRing, int kMost>
 __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams p) {
   __shared__ RowSums sums;
-  extern __shared__ uint4 slots[];
+  constexpr int G = kGroup<TX, TR>, kGroups = kHeld / G;
+  extern __shared__ __align__(16) char slots[];
   const NormArgs& a = p.a;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
@@ -273,14 +253,14 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
   if (worker >= p.workers) return;                 // whole warps of a block of warps
   const int64_t begin = run_start(a.rows, p.workers, worker), end = run_start(a.rows, p.workers, worker + 1);
 
-  const int stage = kRing ? forward_planes<TX, TR>(a) * width : 0, weights = weight_planes(a, false) * width;
-  uint4* const gammas = slots + (weights + kRing * stage) * threadIdx.y;
-  uint4* const g1 = gammas + (a.gamma.ptr ? kWeightPlanes * width : 0);
-  uint4* const ring = gammas + weights;
+  const int stage = kRing ? forward_bytes<TX, TR>(a) * width : 0, weights = weight_bytes(a, false) * width;
+  char* const gammas = slots + (weights + kRing * stage) * threadIdx.y;
+  char* const g1 = gammas + (a.gamma.ptr ? kBytes<float> * width : 0);
+  char* const ring = gammas + weights;
   const auto fetch = [&](int64_t row, int s) {
     if (row < end) {
-      fetch_row<TR>(ring + s * stage, static_cast<const TR*>(a.residual) + row * a.ldr, n, tid, width);
-      if (a.x) fetch_row<TX>(ring + s * stage + kPlanes<TR> * width, static_cast<const TX*>(a.x) + row * a.ldx, n, tid, width);
+      fetch_row<TR, G>(ring + s * stage, static_cast<const TR*>(a.residual) + row * a.ldr, n, tid, width);
+      if (a.x) fetch_row<TX, G>(ring + s * stage + kBytes<TR> * width, static_cast<const TX*>(a.x) + row * a.ldx, n, tid, width);
     }
     copies_commit();
   };
@@ -289,84 +269,96 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
     for (int s = 0; s < kRing - 1; ++s) fetch(begin + s, s);
   }
   if (a.gamma.ptr) {
-    float w[kHeld];
-    load_weight<TX, kVec>(a.gamma, 0, n, tid, width, w);
+    float2 w[kHeld / 2];
+    load_weight<TX, kVec, G>(a.gamma, 0, n, tid, width, w);
     slots_store(gammas, tid, width, w);
   }
   int64_t group = 0, left = 0;                     // rows left of the present group of rows that share a gate
   if (has_g1(a)) {
     group = a.gate.ptr ? begin / a.gate_rows : 0;
     left = a.gate.ptr ? (group + 1) * a.gate_rows - begin : a.rows;
-    form_g1<TX, kVec>(a, group, g1, tid, width);
+    form_g1<TX, kVec, G>(a, group, g1, tid, width);
   }
 
+  constexpr bool kHeldRow = kRing > 0;
   int turn = 0, s = 0;
   for (int64_t t = begin; t < end; ++t) {
-    float v[kHeld], h[kHeld];
-    if constexpr (kRing > 0) {
+    const char* held = ring + s * stage;
+    if constexpr (kHeldRow) {
       fetch(t + kRing - 1, s == 0 ? kRing - 1 : s - 1);
-      const uint4* held = ring + s * stage;
       s = s + 1 == kRing ? 0 : s + 1;
       copies_wait<kRing - 1>();
-      held_row<TR>(held, n, tid, width, h);
-      if (a.x) held_row<TX>(held + kPlanes<TR> * width, n, tid, width, v);
-    } else {
-      load_row<TR, kVec>(static_cast<const TR*>(a.residual) + t * a.ldr, n, tid, width, h);
-      if (a.x) load_row<TX, kVec>(static_cast<const TX*>(a.x) + t * a.ldx, n, tid, width, v);
     }
+    const TX* const row_x = static_cast<const TX*>(a.x) + t * a.ldx;
+    float2 x[kHeld / 2], h[kHeld / 2];
+    float r1 = 1.f;
     if (a.x) {
+      float2 ss = both(0.f);
+#pragma unroll
+      for (int v = 0; v < kGroups; ++v) {
+        take<TX, kVec, kHeldRow, G>(held + kBytes<TR> * width, row_x, v, n, tid, width, x + v * (G / 2));
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) ss = fma2(x[v * (G / 2) + j], x[v * (G / 2) + j], ss);
+      }
       if (a.post_gamma.ptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) ss = fmaf(v[i], v[i], ss);
-        const float r1 = rsqrtf(row_sum(ss, sums, &turn) * inv_n + a.eps);
+        r1 = rsqrtf(row_sum(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
         if (p.r1 && tid == 0) p.r1[t] = r1;
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) v[i] *= r1;
       }
       if (has_g1(a)) {
         if (left == 0) {
-          form_g1<TX, kVec>(a, ++group, g1, tid, width);
+          form_g1<TX, kVec, G>(a, ++group, g1, tid, width);
           left = a.gate_rows;
         }
         --left;
-        float w[kHeld];
-        slots_load(g1, tid, width, w);
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) h[i] = fmaf(a.scale, h[i], v[i] * w[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) h[i] = fmaf(a.scale, h[i], v[i]);
       }
     }
-    if (p.h) store_row<TR, kVec>(static_cast<TR*>(p.h) + t * n, n, tid, width, h);
+    float2 ss = both(0.f);
+#pragma unroll
+    for (int v = 0; v < kGroups; ++v) {
+      take<TR, kVec, kHeldRow, G>(held, static_cast<const TR*>(a.residual) + t * a.ldr, v, n, tid, width, h + v * (G / 2));
+      if (a.x) {
+        if (has_g1(a)) {
+          float2 w[G / 2];
+          slots_load<G>(g1, v, tid, width, w);
+#pragma unroll
+          for (int j = 0; j < G / 2; ++j) x[v * (G / 2) + j] = mul2(mul2(x[v * (G / 2) + j], both(r1)), w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) h[v * (G / 2) + j] = fma2(both(a.scale), h[v * (G / 2) + j], x[v * (G / 2) + j]);
+      }
+#pragma unroll
+      for (int j = 0; j < G / 2; ++j) ss = fma2(h[v * (G / 2) + j], h[v * (G / 2) + j], ss);
+      if (p.h) store_group<TR, kVec, G>(static_cast<TR*>(p.h) + t * n, v, n, tid, width, h + v * (G / 2));
+    }
     if (a.gamma.ptr) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) ss = fmaf(h[i], h[i], ss);
-      const float r2 = rsqrtf(row_sum(ss, sums, &turn) * inv_n + a.eps);
+      const float r2 = rsqrtf(row_sum(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
       if (p.r2 && tid == 0) p.r2[t] = r2;
-      slots_load(gammas, tid, width, v);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) v[i] *= h[i] * r2;
-      store_row<TX, kVec>(static_cast<TX*>(p.y) + t * n, n, tid, width, v);
+      for (int v = 0; v < kGroups; ++v) {
+        float2 w[G / 2];
+        slots_load<G>(gammas, v, tid, width, w);
+#pragma unroll
+        for (int j = 0; j < G / 2; ++j) w[j] = mul2(mul2(h[v * (G / 2) + j], both(r2)), w[j]);
+        store_group<TX, kVec, G>(static_cast<TX*>(p.y) + t * n, v, n, tid, width, w);
+      }
     }
   }
-  if constexpr (kRing > 0) copies_wait<0>();
+  if constexpr (kHeldRow) copies_wait<0>();
 }
 
-template <typename T, bool kVec>
+template <typename T, bool kVec, int G>
 __device__ __forceinline__ void store_weight_grad(void* out, int f32, int64_t first, int n, int tid, int width,
-                                                  const float* f) {
-  if (f32) store_row<float, kVec>(static_cast<float*>(out) + first, n, tid, width, f);
-  else store_row<T, kVec>(static_cast<T*>(out) + first, n, tid, width, f);
+                                                  const float2* f) {
+  if (f32) store_row<float, kVec, G>(static_cast<float*>(out) + first, n, tid, width, f);
+  else store_row<T, kVec, G>(static_cast<T*>(out) + first, n, tid, width, f);
 }
 
 // kRing: rows in shared memory (0: loaded directly).  kFull: a gate or a norm behind the block.
 template <typename TX, typename TR, bool kVec, int kRing, bool kFull, int kMost>
 __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParams p) {
   __shared__ RowSums sums;
-  extern __shared__ uint4 slots[];
+  constexpr int G = kGroup<TX, TR>, kGroups = kHeld / G;
+  extern __shared__ __align__(16) char slots[];
   const NormArgs& a = p.a;
   const NormGrads& g = p.g;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
@@ -376,24 +368,24 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
   if (worker >= p.workers) return;                 // whole warps of a block of warps
   const int64_t begin = run_start(a.rows, p.workers, worker), end = run_start(a.rows, p.workers, worker + 1);
 
-  const int stage = kRing ? backward_planes<TX, TR>(a, g) * width : 0, weights = weight_planes(a, true) * width;
-  uint4* const gammas = slots + (weights + kRing * stage) * threadIdx.y;
-  uint4* const g1 = gammas + (a.gamma.ptr ? kWeightPlanes * width : 0);
-  uint4* const acc_post = g1 + kWeightPlanes * width;        // where there are a gate and a norm behind
-  uint4* const ring = gammas + weights;
-  const int off_dy = g.dh ? kPlanes<TR> * width : 0;
-  const int off_h = off_dy + (g.dy ? kPlanes<TX> * width : 0);
-  const int off_x = off_h + (g.dy ? (g.h ? kPlanes<float> : kPlanes<TR>) * width : 0);
+  const int stage = kRing ? backward_bytes<TX, TR>(a, g) * width : 0, weights = weight_bytes(a, true) * width;
+  char* const gammas = slots + (weights + kRing * stage) * threadIdx.y;
+  char* const g1 = gammas + (a.gamma.ptr ? kBytes<float> * width : 0);
+  char* const acc_post = g1 + kBytes<float> * width;        // where there are a gate and a norm behind
+  char* const ring = gammas + weights;
+  const int off_dy = g.dh ? kBytes<TR> * width : 0;
+  const int off_h = off_dy + (g.dy ? kBytes<TX> * width : 0);
+  const int off_x = off_h + (g.dy ? (g.h ? kBytes<float> : kBytes<TR>) * width : 0);
   const auto fetch = [&](int64_t row, int s) {
     if (row < end) {
-      uint4* to = ring + s * stage;
-      if (g.dh) fetch_row<TR>(to, static_cast<const TR*>(g.dh) + row * g.lddh, n, tid, width);
+      char* to = ring + s * stage;
+      if (g.dh) fetch_row<TR, G>(to, static_cast<const TR*>(g.dh) + row * g.lddh, n, tid, width);
       if (g.dy) {
-        fetch_row<TX>(to + off_dy, static_cast<const TX*>(g.dy) + row * g.lddy, n, tid, width);
-        if (g.h) fetch_row<float>(to + off_h, static_cast<const float*>(g.h) + row * n, n, tid, width);
-        else fetch_row<TR>(to + off_h, static_cast<const TR*>(a.residual) + row * a.ldr, n, tid, width);
+        fetch_row<TX, G>(to + off_dy, static_cast<const TX*>(g.dy) + row * g.lddy, n, tid, width);
+        if (g.h) fetch_row<float, G>(to + off_h, static_cast<const float*>(g.h) + row * n, n, tid, width);
+        else fetch_row<TR, G>(to + off_h, static_cast<const TR*>(a.residual) + row * a.ldr, n, tid, width);
       }
-      if (a.x) fetch_row<TX>(to + off_x, static_cast<const TX*>(a.x) + row * a.ldx, n, tid, width);
+      if (a.x) fetch_row<TX, G>(to + off_x, static_cast<const TX*>(a.x) + row * a.ldx, n, tid, width);
     }
     copies_commit();
   };
@@ -402,22 +394,22 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
     for (int s = 0; s < kRing - 1; ++s) fetch(begin + s, s);
   }
 
-  float acc_gamma[kHeld], acc_s[kFull ? kHeld : 1];
+  float2 acc_gamma[kHeld / 2], acc_s[kFull ? kHeld / 2 : 1];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    acc_gamma[i] = 0.f;
-    if (kFull) acc_s[i] = 0.f;
+  for (int i = 0; i < kHeld / 2; ++i) {
+    acc_gamma[i] = both(0.f);
+    if (kFull) acc_s[i] = both(0.f);
   }
   if (a.gamma.ptr) {
-    float w[kHeld];
-    load_weight<TX, kVec>(a.gamma, 0, n, tid, width, w);
+    float2 w[kHeld / 2];
+    load_weight<TX, kVec, G>(a.gamma, 0, n, tid, width, w);
     slots_store(gammas, tid, width, w);
   }
   int64_t group = 0, left = 0;                     // rows left of the present group of rows that share a gate
   if (kFull) {
     group = a.gate.ptr ? begin / a.gate_rows : 0;
     left = a.gate.ptr ? (group + 1) * a.gate_rows - begin : a.rows;
-    form_g1<TX, kVec>(a, group, g1, tid, width);
+    form_g1<TX, kVec, G>(a, group, g1, tid, width);
     if (a.post_gamma.ptr && a.gate.ptr) slots_store(acc_post, tid, width, acc_gamma);
   }
   float next_r1 = kFull && a.post_gamma.ptr && begin < end ? g.r1[begin] : 1.f;
@@ -425,151 +417,148 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
 
   int turn = 0, s = 0;
   for (int64_t t = begin; t < end; ++t) {
-    float d[kHeld];
     const float r1 = next_r1, r2 = next_r2;
     if (t + 1 < end) {
       if (kFull && a.post_gamma.ptr) next_r1 = g.r1[t + 1];
       if (g.dy) next_r2 = g.r2[t + 1];
     }
-    const uint4* held = ring + s * stage;
-    if constexpr (kRing > 0) {
+    constexpr bool kHeldRow = kRing > 0;
+    const char* held = ring + s * stage;
+    if constexpr (kHeldRow) {
       fetch(t + kRing - 1, s == 0 ? kRing - 1 : s - 1);
       s = s + 1 == kRing ? 0 : s + 1;
       copies_wait<kRing - 1>();
     }
-    constexpr bool kHeldRow = kRing > 0;
     const TX* const row_x = static_cast<const TX*>(a.x) + t * a.ldx;
-    const TX* const row_dy = static_cast<const TX*>(g.dy) + t * g.lddy;
-    const TR* const row_dh = static_cast<const TR*>(g.dh) + t * g.lddh;
     // The row is gone through in groups of eight values, and inputs are read again rather than kept: what stays in
     // registers over a barrier are the two sums of the weights' gradients and two values a column.
-    float n2[kHeld];
+    float2 d[kHeld / 2], n2[kHeld / 2];
     if (g.dy) {
-      float dot = 0.f;
+      float2 dot = both(0.f);
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        float f[8], w[8];
-        float* const h = n2 + 8 * v;
+      for (int v = 0; v < kGroups; ++v) {
+        float2 f[G / 2], w[G / 2];
+        float2* const h = n2 + v * (G / 2);
         if (g.h) {
-          take8<float, kVec, kHeldRow>(held + off_h, static_cast<const float*>(g.h) + t * n, v, n, tid, width, h);
+          take<float, kVec, kHeldRow, G>(held + off_h, static_cast<const float*>(g.h) + t * n, v, n, tid, width, h);
         } else {
-          take8<TR, kVec, kHeldRow>(held + off_h, static_cast<const TR*>(a.residual) + t * a.ldr, v, n, tid, width, h);
+          take<TR, kVec, kHeldRow, G>(held + off_h, static_cast<const TR*>(a.residual) + t * a.ldr, v, n, tid, width, h);
           if (a.x) {
-            take8<TX, kVec, kHeldRow>(held + off_x, row_x, v, n, tid, width, f);
+            take<TX, kVec, kHeldRow, G>(held + off_x, row_x, v, n, tid, width, f);
             if (kFull) {
-              slots_load8(g1, v, tid, width, w);
+              slots_load<G>(g1, v, tid, width, w);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] *= r1 * w[j];
+              for (int j = 0; j < G / 2; ++j) f[j] = mul2(mul2(f[j], both(r1)), w[j]);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = fmaf(a.scale, h[j], f[j]);
+            for (int j = 0; j < G / 2; ++j) h[j] = fma2(both(a.scale), h[j], f[j]);
           }
         }
-        take8<TX, kVec, kHeldRow>(held + off_dy, row_dy, v, n, tid, width, f);
-        slots_load8(gammas, v, tid, width, w);
+        take<TX, kVec, kHeldRow, G>(held + off_dy, static_cast<const TX*>(g.dy) + t * g.lddy, v, n, tid, width, f);
+        slots_load<G>(gammas, v, tid, width, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          h[j] *= r2;
-          acc_gamma[8 * v + j] = fmaf(f[j], h[j], acc_gamma[8 * v + j]);
-          d[8 * v + j] = f[j] * w[j];
-          dot = fmaf(d[8 * v + j], h[j], dot);
+        for (int j = 0; j < G / 2; ++j) {
+          h[j] = mul2(h[j], both(r2));
+          acc_gamma[v * (G / 2) + j] = fma2(f[j], h[j], acc_gamma[v * (G / 2) + j]);
+          d[v * (G / 2) + j] = mul2(f[j], w[j]);
+          dot = fma2(d[v * (G / 2) + j], h[j], dot);
         }
       }
-      const float pull = -r2 * inv_n * row_sum(dot, sums, &turn);
+      const float pull = -r2 * inv_n * row_sum(dot.x + dot.y, sums, &turn);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) d[i] = fmaf(r2, d[i], pull * n2[i]);
+      for (int i = 0; i < kHeld / 2; ++i) d[i] = fma2(both(r2), d[i], mul2(both(pull), n2[i]));
     } else {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) d[i] = 0.f;
+      for (int i = 0; i < kHeld / 2; ++i) d[i] = both(0.f);
     }
-    float dot = 0.f;
+    float2 dot = both(0.f);
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      float f[8], w[8];
+    for (int v = 0; v < kGroups; ++v) {
+      float2 f[G / 2], w[G / 2];
       if (g.dh) {
-        take8<TR, kVec, kHeldRow>(held, row_dh, v, n, tid, width, f);
+        take<TR, kVec, kHeldRow, G>(held, static_cast<const TR*>(g.dh) + t * g.lddh, v, n, tid, width, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[8 * v + j] += f[j];
+        for (int j = 0; j < G / 2; ++j) d[v * (G / 2) + j] = add2(d[v * (G / 2) + j], f[j]);
       }
       if (g.dresidual) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = a.scale * d[8 * v + j];
-        put8<TR, kVec>(static_cast<TR*>(g.dresidual) + t * n, v, n, tid, width, f);
+        for (int j = 0; j < G / 2; ++j) f[j] = mul2(both(a.scale), d[v * (G / 2) + j]);
+        store_group<TR, kVec, G>(static_cast<TR*>(g.dresidual) + t * n, v, n, tid, width, f);
       }
       if constexpr (kFull) {
-        take8<TX, kVec, kHeldRow>(held + off_x, row_x, v, n, tid, width, f);
-        slots_load8(g1, v, tid, width, w);
+        take<TX, kVec, kHeldRow, G>(held + off_x, row_x, v, n, tid, width, f);
+        slots_load<G>(g1, v, tid, width, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[j] *= r1;
-          acc_s[8 * v + j] = fmaf(d[8 * v + j], f[j], acc_s[8 * v + j]);
-          d[8 * v + j] *= w[j];
-          dot = fmaf(d[8 * v + j], f[j], dot);
+        for (int j = 0; j < G / 2; ++j) {
+          f[j] = mul2(f[j], both(r1));
+          acc_s[v * (G / 2) + j] = fma2(d[v * (G / 2) + j], f[j], acc_s[v * (G / 2) + j]);
+          d[v * (G / 2) + j] = mul2(d[v * (G / 2) + j], w[j]);
+          dot = fma2(d[v * (G / 2) + j], f[j], dot);
         }
       }
     }
     if (kFull && a.post_gamma.ptr) {
       // n1 = r1 * x once more
-      const float pull = -r1 * r1 * inv_n * row_sum(dot, sums, &turn);
+      const float pull = -r1 * r1 * inv_n * row_sum(dot.x + dot.y, sums, &turn);
       if (g.dx) {
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-          float f[8];
-          take8<TX, kVec, kHeldRow>(held + off_x, row_x, v, n, tid, width, f);
+        for (int v = 0; v < kGroups; ++v) {
+          float2 f[G / 2];
+          take<TX, kVec, kHeldRow, G>(held + off_x, row_x, v, n, tid, width, f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = fmaf(r1, d[8 * v + j], pull * f[j]);
-          put8<TX, kVec>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, f);
+          for (int j = 0; j < G / 2; ++j) f[j] = fma2(both(r1), d[v * (G / 2) + j], mul2(both(pull), f[j]));
+          store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, f);
         }
       }
     } else if (g.dx) {
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) put8<TX, kVec>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, d + 8 * v);
+      for (int v = 0; v < kGroups; ++v) store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, d + v * (G / 2));
     }
     if constexpr (kFull) {
       if (--left == 0 || t + 1 == end) {
         if (a.gate.ptr) {
           // The group's last row here: dgate is whole if this run held all of the group, else a part.
           if (a.post_gamma.ptr) {
-            float w[kHeld];
-            load_weight<TX, kVec>(a.gate, group * n, n, tid, width, w);
-            slots_load(acc_post, tid, width, d);
+            float2 w[kHeld / 2], sum[kHeld / 2];
+            load_weight<TX, kVec, G>(a.gate, group * n, n, tid, width, w);
+            slots_load<kHeld>(acc_post, 0, tid, width, sum);
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) d[i] = fmaf(w[i], acc_s[i], d[i]);
-            slots_store(acc_post, tid, width, d);
-            load_weight<TX, kVec>(a.post_gamma, 0, n, tid, width, w);
+            for (int i = 0; i < kHeld / 2; ++i) sum[i] = fma2(w[i], acc_s[i], sum[i]);
+            slots_store(acc_post, tid, width, sum);
+            load_weight<TX, kVec, G>(a.post_gamma, 0, n, tid, width, w);
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) acc_s[i] *= w[i];
+            for (int i = 0; i < kHeld / 2; ++i) acc_s[i] = mul2(acc_s[i], w[i]);
           }
           if (g.dgate) {
             if (group * a.gate_rows >= begin && (group + 1) * a.gate_rows <= end) {
-              store_weight_grad<TX, kVec>(g.dgate, a.gate.f32, group * n, n, tid, width, acc_s);
+              store_weight_grad<TX, kVec, G>(g.dgate, a.gate.f32, group * n, n, tid, width, acc_s);
             } else {
               const int slot = group * a.gate_rows <= begin ? 0 : 1;
-              store_row<float, kVec>(p.part_gate + (static_cast<int64_t>(worker) * 2 + slot) * n, n, tid, width, acc_s);
+              store_row<float, kVec, G>(p.part_gate + (static_cast<int64_t>(worker) * 2 + slot) * n, n, tid, width, acc_s);
             }
           }
 #pragma unroll
-          for (int i = 0; i < kHeld; ++i) acc_s[i] = 0.f;
-          if (t + 1 < end) form_g1<TX, kVec>(a, ++group, g1, tid, width);
+          for (int i = 0; i < kHeld / 2; ++i) acc_s[i] = both(0.f);
+          if (t + 1 < end) form_g1<TX, kVec, G>(a, ++group, g1, tid, width);
           left = a.gate_rows;
         }
       }
     }
   }
   if constexpr (kRing > 0) copies_wait<0>();
-  if (p.part_gamma) store_row<float, kVec>(p.part_gamma + static_cast<int64_t>(worker) * n, n, tid, width, acc_gamma);
+  if (p.part_gamma) store_row<float, kVec, G>(p.part_gamma + static_cast<int64_t>(worker) * n, n, tid, width, acc_gamma);
   if constexpr (kFull) {
     if (p.part_post) {
-      if (a.gate.ptr) slots_load(acc_post, tid, width, acc_s);
-      store_row<float, kVec>(p.part_post + static_cast<int64_t>(worker) * n, n, tid, width, acc_s);
+      if (a.gate.ptr) slots_load<kHeld>(acc_post, 0, tid, width, acc_s);
+      store_row<float, kVec, G>(p.part_post + static_cast<int64_t>(worker) * n, n, tid, width, acc_s);
     }
   }
 }
 
 // Adds the workers' parts in their order: blockIdx.y 0 gamma, 1 post_gamma, 2.. the groups of gate rows.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormParams p) {
-  __shared__ float part[32][33];
+__global__ void __launch_bounds__(256) norm_reduce_kernel(const NormParams p) {
+  __shared__ float part[8][32];
   const NormArgs& a = p.a;
   const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5, n = a.hidden;
   const int col = blockIdx.x * 32 + lane;
@@ -597,18 +586,22 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormParams p) {
     if (src == nullptr || out == nullptr) continue;
     float sum = 0.f;
     if (col < n) {
-#pragma unroll 4
-      for (int w = first + strip; w < last; w += 32) {
-        const float* at = src + w * step;
-        if (what >= 2 && group * a.gate_rows > run_start(a.rows, p.workers, w)) at += n;
-        sum += at[col];
+      // Only the first of them can have begun with another group: its part stands in the second place.
+      if (strip == 0 && what >= 2) {
+        sum = src[first * step + (group * a.gate_rows > run_start(a.rows, p.workers, first) ? n : 0) + col];
+        ++first;
+      } else if (what >= 2) {
+        ++first;
       }
+      const float* at = src + (first + strip) * step + col;
+#pragma unroll 8
+      for (int w = first + strip; w < last; w += 8, at += 8 * step) sum += *at;
     }
     part[strip][lane] = sum;
     __syncthreads();
     if (strip == 0 && col < n) {
 #pragma unroll
-      for (int s = 1; s < 32; ++s) sum += part[s][lane];
+      for (int s = 1; s < 8; ++s) sum += part[s][lane];
       if (f32) static_cast<float*>(out)[group * n + col] = sum;
       else static_cast<T*>(out)[group * n + col] = from_f32<T>(sum);
     }
@@ -639,7 +632,8 @@ bool aligned(const void* p, int64_t ld, int bytes) {
 bool aligned(const Weight& w, int64_t hidden, DType t) { return aligned(w.ptr, hidden, w.f32 ? 4 : dtype_bytes(t)); }
 
 bool inputs_aligned(const NormArgs& a) {
-  return a.hidden % 8 == 0 && aligned(a.x, a.ldx, dtype_bytes(a.xt)) && aligned(a.residual, a.ldr, dtype_bytes(a.rt)) &&
+  const bool wide = a.xt == DType::kF32 || a.rt == DType::kF32;
+  return a.hidden % (wide ? 4 : 8) == 0 && aligned(a.x, a.ldx, dtype_bytes(a.xt)) && aligned(a.residual, a.ldr, dtype_bytes(a.rt)) &&
          aligned(a.gamma, a.hidden, a.xt) && aligned(a.post_gamma, a.hidden, a.xt) && aligned(a.gate, a.hidden, a.xt);
 }
 
@@ -679,8 +673,8 @@ template <typename TX, typename TR, int kMost>
 void forward_typed(NormParams& p, bool vec, cudaStream_t stream) {
   const Shape s = shape_of(p.a.hidden);
   const int threads = static_cast<int>(s.block.x * s.block.y);
-  const size_t weights = static_cast<size_t>(weight_planes(p.a, false)) * 16 * threads;
-  const size_t row = static_cast<size_t>(forward_planes<TX, TR>(p.a)) * 16 * threads;
+  const size_t weights = static_cast<size_t>(weight_bytes(p.a, false)) * threads;
+  const size_t row = static_cast<size_t>(forward_bytes<TX, TR>(p.a)) * threads;
   const int ring = vec ? ring_rows(weights, row, 3, threads < 512 ? 768 / threads : 1) : 0;
   if (ring == 3) launch_norm(norm_forward_kernel<TX, TR, true, 3, kMost>, p, true, weights + 3 * row, stream);
   else if (ring == 2) launch_norm(norm_forward_kernel<TX, TR, true, 2, kMost>, p, true, weights + 2 * row, stream);
@@ -692,8 +686,8 @@ template <typename TX, typename TR, bool kFull, int kMost>
 void backward_full(NormParams& p, bool vec, cudaStream_t stream) {
   const Shape s = shape_of(p.a.hidden);
   const int threads = static_cast<int>(s.block.x * s.block.y);
-  const size_t weights = static_cast<size_t>(weight_planes(p.a, true)) * 16 * threads;
-  const size_t row = static_cast<size_t>(backward_planes<TX, TR>(p.a, p.g)) * 16 * threads;
+  const size_t weights = static_cast<size_t>(weight_bytes(p.a, true)) * threads;
+  const size_t row = static_cast<size_t>(backward_bytes<TX, TR>(p.a, p.g)) * threads;
   const int ring = vec ? ring_rows(weights, row, 3, threads < 512 ? 512 / threads : 1) : 0;
   if (ring == 3) launch_norm(norm_backward_kernel<TX, TR, true, 3, kFull, kMost>, p, false, weights + 3 * row, stream);
   else if (ring == 2) launch_norm(norm_backward_kernel<TX, TR, true, 2, kFull, kMost>, p, false, weights + 2 * row, stream);
@@ -762,7 +756,7 @@ void norm_backward(const NormArgs& a, const NormGrads& g, cudaStream_t stream) {
   if (g.dgamma || g.dpost_gamma || g.dgate) {
     const int64_t targets = 2 + (g.dgate ? a.rows / a.gate_rows : 0);
     const dim3 grid((a.hidden + 31) / 32, static_cast<unsigned>(targets < 1024 ? targets : 1024));
-    PCCL_BLOCK_TYPES(a.xt, T, norm_reduce_kernel<T><<<grid, 1024, 0, stream>>>(p))
+    PCCL_BLOCK_TYPES(a.xt, T, norm_reduce_kernel<T><<<grid, 256, 0, stream>>>(p))
     PCCL_CUDA(cudaGetLastError());
   }
 }
