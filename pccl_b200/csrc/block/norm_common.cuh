@@ -1,0 +1,306 @@
+// What the two kernels of the block norms share: columns, the ring of rows in shared memory, sums over a row.
+//
+// Both kernels are bound by memory, and what keeps memory waiting is a row's own chain: load, sum over the row,
+// barrier, use, perhaps a second sum.  So the coming rows are on their way into a ring in shared memory (cp.async,
+// which holds no registers) while a block works on the present one.  Four ways of reading a row:
+//
+//   kRing     rows aligned to 16 bytes: every thread copies the columns it will use into slots of its own, so no
+//             barrier is needed to read them;
+//   kWindow   rows that begin anywhere (odd sizes, cut views): the block copies the 16-byte blocks that cover the
+//             row and picks the values out of shared memory;
+//   kDirect, kScalar   rows too long for the ring, loaded where they are used, by 16 bytes or one by one.
+#pragma once
+#include "../common/launch.h"
+#include "../common/util.h"
+#include "../engine/cuda_driver.h"
+#include "vec.cuh"
+
+namespace pccl {
+namespace block {
+namespace norm {
+
+constexpr int kHeld = 16;                      // values a thread holds of its row
+enum Mode : int { kRing = 0, kWindow = 1, kDirect = 2, kScalar = 3 };
+constexpr bool aligned_mode(int m) { return m == kRing || m == kDirect; }
+
+// A thread's values stand in groups of consecutive columns, as many as 16 bytes of the widest type hold: a warp then
+// touches whole 32-byte sectors in every access.  (Eight columns of 32 bits a thread, as two accesses 32 bytes apart
+// from lane to lane, moved every sector twice: 126 us instead of 84 for 4100 x 8192 backwards.)
+template <typename TX, typename TR> constexpr int kGroup = sizeof(TX) == 4 || sizeof(TR) == 4 ? 4 : 8;
+
+struct NormParams {
+  NormArgs a;
+  NormGrads g;
+  void* h;
+  void* y;
+  float* r1;
+  float* r2;
+  float* part_gamma;          // [workers][hidden]
+  float* part_post;           // [workers][hidden]
+  float* part_gate;           // [workers][2][hidden]: the run's first group of rows, its last one
+  int workers;                // blocks, each with a run of consecutive rows
+  int ring;                   // rows in shared memory
+};
+
+// Column of value j of group v held by a thread: G in a row where rows are aligned, else a thread's values stand a
+// whole row of threads apart, so that neighbours read neighbours.
+template <bool kVec, int G> __device__ __forceinline__ int column(int v, int j, int tid, int width) {
+  return kVec ? (v * width + tid) * G + j : (v * G + j) * width + tid;
+}
+
+// G values as they lie in memory.
+template <typename T, int G> struct alignas(G * sizeof(T) > 16 ? 16 : G * sizeof(T)) Raw { uint32_t w[G * sizeof(T) / 4]; };
+
+template <typename T, int G> __device__ __forceinline__ void unpack(const Raw<T, G>& r, float2* f) {
+#pragma unroll
+  for (int i = 0; i < G / 2; ++i) {
+    if constexpr (sizeof(T) == 4) f[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else unpack2(r.w[i], &f[i].x, T());
+  }
+}
+template <typename T, int G> __device__ __forceinline__ Raw<T, G> pack(const float2* f) {
+  Raw<T, G> r;
+#pragma unroll
+  for (int i = 0; i < G / 2; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r.w[2 * i] = __float_as_uint(f[i].x);
+      r.w[2 * i + 1] = __float_as_uint(f[i].y);
+    } else {
+      r.w[i] = pack2(f[i].x, f[i].y, T());
+    }
+  }
+  return r;
+}
+
+// The values of group v, from the row itself.
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void load_group(const T* row, int v, int hidden, int tid, int width, float2* to) {
+  if constexpr (kVec) {
+    const int at = (v * width + tid) * G;
+    if (at < hidden) {
+      unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(row + at), to);
+    } else {
+#pragma unroll
+      for (int j = 0; j < G / 2; ++j) to[j] = make_float2(0.f, 0.f);
+    }
+  } else {
+    float* f = reinterpret_cast<float*>(to);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int at = column<false, G>(v, j, tid, width);
+      f[j] = at < hidden ? to_f32<T>(row[at]) : 0.f;
+    }
+  }
+}
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void store_group(T* row, int v, int hidden, int tid, int width, const float2* from) {
+  if constexpr (kVec) {
+    const int at = (v * width + tid) * G;
+    if (at < hidden) *reinterpret_cast<Raw<T, G>*>(row + at) = pack<T, G>(from);
+  } else {
+    const float* f = reinterpret_cast<const float*>(from);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int at = column<false, G>(v, j, tid, width);
+      if (at < hidden) row[at] = from_f32<T>(f[j]);
+    }
+  }
+}
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void store_row(T* row, int hidden, int tid, int width, const float2* f) {
+#pragma unroll
+  for (int v = 0; v < kHeld / G; ++v) store_group<T, kVec, G>(row, v, hidden, tid, width, f + v * (G / 2));
+}
+// A weight vector is of the activations' type or of 32 bits.
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void load_weight(const Weight& w, int64_t first, int hidden, int tid, int width, float2* f) {
+#pragma unroll
+  for (int v = 0; v < kHeld / G; ++v) {
+    if (w.f32) load_group<float, kVec, G>(static_cast<const float*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
+    else load_group<T, kVec, G>(static_cast<const T*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
+  }
+}
+
+// ---- ring ------------------------------------------------------------------------------------------------
+// A thread's share of a row of T: kHeld values.  A weight's slots and (mode kRing) a row's stand group by group, the
+// threads' next to one another: a warp's copies then fill whole lines of shared memory.  (With each thread's slots
+// in one piece the copies of neighbours went to different lines, and every kernel here took a quarter longer.)
+template <typename T> constexpr int kBytes = kHeld * static_cast<int>(sizeof(T));
+
+// The first `size` of kSize bytes (8 or 16), and zeros for the rest.
+template <int kSize> __device__ __forceinline__ void copy_async(char* to, const void* from, int size) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (kSize == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(size) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until at most `left` of the groups committed last are under way.
+__device__ __forceinline__ void copies_wait(int left) {
+  if (left <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
+
+template <typename T, int G>
+__device__ __forceinline__ void fetch_share(char* slot, const T* row, int hidden, int tid, int width) {
+#pragma unroll
+  for (int v = 0; v < kHeld / G; ++v) {
+    const int at = (v * width + tid) * G;
+    const bool beyond = at >= hidden;
+    constexpr int kSize = G * static_cast<int>(sizeof(T));
+    copy_async<kSize>(slot + (v * width + tid) * kSize, row + (beyond ? 0 : at), beyond ? 0 : kSize);
+  }
+}
+
+// Bytes of a window for any row of T.
+template <typename T> __host__ __device__ constexpr int window_bytes(int hidden) {
+  return (hidden * static_cast<int>(sizeof(T)) + 15) / 16 * 16 + 16;
+}
+// The 16-byte blocks that cover the row.  The first may begin with values in front of it: such a block holds a value
+// of the row, and allocations begin at multiples of 256 bytes, so all of it is theirs.  Nothing is read behind.
+template <typename T>
+__device__ __forceinline__ void fetch_window(char* window, const T* row, int hidden, int tid, int width) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(row), end = begin + static_cast<uintptr_t>(hidden) * sizeof(T);
+  const uintptr_t first = begin & ~static_cast<uintptr_t>(15);
+  const int blocks = static_cast<int>((end - first + 15) / 16);
+  for (int i = tid; i < blocks; i += width) {
+    const uintptr_t from = first + static_cast<uintptr_t>(i) * 16;
+    copy_async<16>(window + i * 16, reinterpret_cast<const void*>(from), static_cast<int>(min(end - from, static_cast<uintptr_t>(16))));
+  }
+}
+
+// Group v of a row of T: `slot` is the row's place in the ring, or the window.
+template <typename T, int kMode, int G>
+__device__ __forceinline__ void take(const char* slot, const T* row, int v, int hidden, int tid, int width, float2* to) {
+  if constexpr (kMode == kRing) {
+    unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(slot + (v * width + tid) * static_cast<int>(G * sizeof(T))), to);
+  } else if constexpr (kMode == kWindow) {
+    const T* at = reinterpret_cast<const T*>(slot + (reinterpret_cast<uintptr_t>(row) & 15));
+    load_group<T, false, G>(at, v, hidden, tid, width, to);
+  } else {
+    load_group<T, kMode == kDirect, G>(row, v, hidden, tid, width, to);
+  }
+}
+
+// Sum over the block; `sums` alternates between two sets so that one barrier a call is enough.  Sets are cleared
+// once (row_sum_clear), so that whole groups of four can be read.
+struct __align__(16) RowSums { float set[2][32]; };
+__device__ __forceinline__ void row_sum_clear(RowSums& sums) {
+  if (blockDim.x == 32) return;
+  if (threadIdx.x < 64) (&sums.set[0][0])[threadIdx.x] = 0.f;
+  __syncthreads();
+}
+__device__ __forceinline__ float row_sum(float v, RowSums& sums, int* turn) {
+  v = warp_sum(v);
+  if (blockDim.x == 32) return v;
+  float* s = sums.set[*turn];
+  *turn ^= 1;
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(s + w);
+    v += (q.x + q.y) + (q.z + q.w);
+  }
+  return v;
+}
+
+// A weight's slots: kHeld 32-bit values, four to an access.
+__device__ __forceinline__ void slots_store(char* slot, int tid, int width, const float2* f) {
+#pragma unroll
+  for (int i = 0; i < kHeld / 4; ++i)
+    reinterpret_cast<float4*>(slot)[i * width + tid] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
+}
+template <int G> __device__ __forceinline__ void slots_load(const char* slot, int v, int tid, int width, float2* f) {
+#pragma unroll
+  for (int i = 0; i < G / 4; ++i) {
+    const float4 q = reinterpret_cast<const float4*>(slot)[(v * (G / 4) + i) * width + tid];
+    f[2 * i] = make_float2(q.x, q.y);
+    f[2 * i + 1] = make_float2(q.z, q.w);
+  }
+}
+
+// g1 = post_gamma * gate of one group of rows into its slots (what is absent counts as 1).
+template <typename T, bool kVec, int G>
+__device__ __forceinline__ void form_g1(const NormArgs& a, int64_t group, char* slot, int tid, int width) {
+  float2 f[kHeld / 2], w[kHeld / 2];
+  if (a.post_gamma.ptr) load_weight<T, kVec, G>(a.post_gamma, 0, a.hidden, tid, width, f);
+  if (a.gate.ptr) {
+    load_weight<T, kVec, G>(a.gate, group * a.hidden, a.hidden, tid, width, w);
+#pragma unroll
+    for (int i = 0; i < kHeld / 2; ++i) f[i] = a.post_gamma.ptr ? mul2(f[i], w[i]) : w[i];
+  }
+  slots_store(slot, tid, width, f);
+}
+
+// First row of worker w's run; w = workers gives the number of rows.
+__device__ __forceinline__ int64_t run_start(int64_t rows, int workers, int w) {
+  return rows / workers * w + min(static_cast<int64_t>(w), rows % workers);
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+inline int threads_of(int hidden) { return ((hidden + kHeld - 1) / kHeld + 31) / 32 * 32; }
+
+inline int sm_count() {
+  int dev = 0, sms = 0;
+  PCCL_CUDA(cudaGetDevice(&dev));
+  PCCL_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  return sms;
+}
+
+inline bool has_g1(const NormArgs& a) { return a.post_gamma.ptr || a.gate.ptr; }
+
+inline bool aligned(const void* p, int64_t ld, int bytes) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0);
+}
+inline bool aligned(const Weight& w, int64_t hidden, DType t) { return aligned(w.ptr, hidden, w.f32 ? 4 : dtype_bytes(t)); }
+inline bool inputs_aligned(const NormArgs& a) {
+  const bool wide = a.xt == DType::kF32 || a.rt == DType::kF32;
+  return a.hidden % (wide ? 4 : 8) == 0 && aligned(a.x, a.ldx, dtype_bytes(a.xt)) && aligned(a.residual, a.ldr, dtype_bytes(a.rt)) &&
+         aligned(a.gamma, a.hidden, a.xt) && aligned(a.post_gamma, a.hidden, a.xt) && aligned(a.gate, a.hidden, a.xt);
+}
+
+// Shared memory of an SM, and the most of one block (less what the kernels themselves and the driver keep).
+constexpr size_t kSmemSm = 228 * 1024, kSmemBlock = 226 * 1024, kSmemKept = 1024 + sizeof(RowSums);
+constexpr int kMostRing = 4;
+
+// Shared memory of a block with `rows` rows in the ring.
+struct RingSize {
+  int threads;
+  int weights, share;         // bytes a thread: weights, its share of one row (kRing)
+  int window;                 // bytes of one row's windows
+  size_t bytes(int mode, int rows) const {
+    return static_cast<size_t>(weights + (mode == kRing ? rows * share : 0)) * threads +
+           (mode == kWindow ? static_cast<size_t>(rows) * window : 0);
+  }
+  // As many rows as leave `blocks` blocks on an SM, at least two; 0 where two do not fit into one.
+  int rows(int mode, int blocks) const {
+    for (int r = kMostRing; r > 2; --r)
+      if ((bytes(mode, r) + kSmemKept) * blocks <= kSmemSm && bytes(mode, r) <= kSmemBlock) return r;
+    return bytes(mode, 2) <= kSmemBlock ? 2 : 0;
+  }
+};
+// Registers let 512 threads of 128 registers (or 1024 of 64) share an SM.
+inline int blocks_per_sm(int threads) { return threads < 512 ? 512 / threads : 1; }
+
+// The mode for these rows; *ring and *smem go with it.
+inline int choose_mode(const RingSize& size, bool vec, int* ring, size_t* smem) {
+  int mode = vec ? kRing : kWindow;
+  *ring = size.rows(mode, blocks_per_sm(size.threads));
+  if (*ring == 0) mode = vec ? kDirect : kScalar;
+  *smem = size.bytes(mode, *ring);
+  return mode;
+}
+
+template <class Kernel> void launch(Kernel kernel, const NormParams& p, int threads, size_t smem, cudaStream_t stream) {
+  if (smem > 40 * 1024)
+    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  kernel<<<p.workers, threads, smem, stream>>>(p);
+}
+
+}  // namespace norm
+}  // namespace block
+}  // namespace pccl
