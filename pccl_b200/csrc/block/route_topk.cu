@@ -6,15 +6,17 @@
 //   w_k = scale * p_k / sum p  (or scale * p_k);
 //   rows[t][k] = offsets[idx] + number of earlier tokens that chose the same expert.
 //
-// One warp per token, expert e in lane e / NE, so that the lowest lane holds the lowest number and a tie is
-// decided by the first set bit of a ballot.  Scores are compared as unsigned keys of the same order (one
-// redux.sync a round).
+// Up to 8 experts one thread takes a token (16384 tokens, 8 experts: 19 us with a warp each); above that one warp,
+// expert e in lane e / NE, so that the lowest lane holds the lowest number and a tie is decided by the first set bit of
+// a ballot.  Scores are compared as unsigned keys of the same order (one redux.sync a round); a lane keeps its keys
+// sorted, so that a round costs the winner a shift.  Many tokens are bound by instructions, not by the 4 bytes a
+// score that they read.
 //
 // The order of two scores is part of the answer, and 32 bits cannot tell scores apart that differ by less than
 // their rounding.  Without a bias the order is that of the logits and needs no arithmetic.  With one, the choice
 // is made in 32 bits together with the runner-up; where any two neighbours of the sorted choice (or the last
-// group kept and the first dropped) are nearer than the error bound of the arithmetic, the warp repeats the
-// token in 64 bits.  Equal logits with equal biases are a true tie and need no repeat.
+// group kept and the first dropped) are nearer than the error bound of the arithmetic, the token is chosen again
+// in 64 bits.  Equal logits with equal biases are a true tie and need no repeat.
 //
 // Rows in expert order need no atomics whose order matters: a block of consecutive tokens marks its choices as
 // bits in shared memory ([expert][token]), a choice's rank is a population count, and the blocks' counts
@@ -30,16 +32,19 @@ namespace block {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMostThreads = 1024;
+constexpr int kThreadExperts = 8;             // up to so many experts a thread takes a token
 
 struct RouteParams {
   RouteArgs a;
   const float* dweights;
   void* dlogits;
-  uint16_t* counts;           // [blocks][experts]: choices per expert of one block's tokens
+  uint16_t* counts;           // [blocks][pitch]: choices per expert of one block's tokens
+  int pitch;                  // experts, rounded up to even
   int tokens_per_block, words;
+  int vec;                    // rows of logits can be read a lane's (or thread's) share at once
+  int lanes;                  // lanes that share a group, a power of two; 0: groups do not divide so
 };
 
 // Unsigned keys in the order of the values; 0 stands below every value, infinities included.
@@ -69,114 +74,192 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
+template <typename K> __device__ __forceinline__ K larger(K a, K b) { return a > b ? a : b; }
+template <typename K> __device__ __forceinline__ K smaller(K a, K b) { return a > b ? b : a; }
 
 // NaN counts as the lowest logit; +infinity as the largest finite one, so that no score is a NaN.  The sum with
 // zero turns -0 into +0: the two are equal and their keys have to be.
-__device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, 3.402823466e38f) + 0.f; }
+__device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f) + 0.f; }
 
-// Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Lane
-// i < top_k returns the i-th expert; *near is set where two scores that decide something differ by no more than
-// tau (+ 2^-21 of their size).
+__device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
+// For the choice alone.
+__device__ __forceinline__ float quick_sigmoid(float l) { return __fdividef(1.f, 1.f + __expf(-l)); }
+
+// Bound of the difference of two scores' errors; __expf(x) is off by (2 + 1.2 |x|) 2^-23 of itself.  Sigmoid:
+// p (1 - p) times that is at most 0.7 * 2^-23, the sum and quotient add 2^-22.  Softmax: of the row's largest
+// probability, exponential 5 * 2^-24 (|x| e^-|x| < 0.37), the sum over a lane and the warp (n + 5) 2^-24 and its terms'
+// 5 * 2^-24, quotient and product 3 * 2^-24.
+__device__ __forceinline__ float score_error(bool sigmoid_scores, int n, float largest) {
+  return sigmoid_scores ? 0x1p-20f : static_cast<float>(n + 20) * 0x1p-23f * largest;
+}
+
+// ---- a warp per token ------------------------------------------------------------------------------------------
+// Largest first, among equals the lowest number first (comparators keep equals in place only between neighbours, so
+// numbers take part in the comparison where keys are equal).
+template <typename Key, int NE>
+__device__ __forceinline__ void sort_lane(Key (&key)[NE], uint32_t (&num)[NE]) {
+  const auto order = [&](int i, int j) {
+    const bool swap = key[j] > key[i] || (key[j] == key[i] && num[j] < num[i]);
+    const Key k = swap ? key[j] : key[i];
+    const uint32_t n = swap ? num[j] : num[i];
+    key[j] = swap ? key[i] : key[j];
+    num[j] = swap ? num[i] : num[j];
+    key[i] = k;
+    num[i] = n;
+  };
+  // Batcher's odd-even merge sort.
+#pragma unroll
+  for (int p = 1; p < NE; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < NE; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < NE && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(i + j, i + j + k);
+}
+
+// Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Expert
+// numbers go to picked[0 .. top_k - 1] in shared memory (with `check` the runner-up's behind them).  Returns whether
+// two scores that decide something differ by no more than tau (+ 2^-21 of their size): bit 0 in lane i for choices i and
+// i + 1, bit 1 for the groups.
 template <typename F, int NE>
-__device__ __forceinline__ int choose(const RouteArgs& a, const F (&s)[NE], float tau, bool check, const float (&l)[NE],
-                                      const float (&bias)[NE], bool* near) {
+__device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], float tau, bool check, const float (&l)[NE],
+                                       uint16_t* picked) {
   using Key = decltype(key_of(F()));
+  constexpr bool kSorted = NE <= 8;               // sorting 16 or 32 keys costs more than a few rounds of search
+  const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   Key key[NE];
+  uint32_t num[NE];
 #pragma unroll
-  for (int j = 0; j < NE; ++j) key[j] = lane * NE + j < a.experts ? key_of(s[j]) : Key(0);
-  bool close = false;
+  for (int j = 0; j < NE; ++j) {
+    key[j] = lane * NE + j < a.experts ? key_of(s[j]) : Key(0);
+    num[j] = j;
+  }
+  int close = 0;
+  const bool grouped = a.top_groups < a.groups;
+  const bool by_logit = a.bias == nullptr && a.top2 && grouped;   // s is not the logits here
 
-  if (a.top_groups < a.groups) {
+  if (grouped) {
     const int size = a.experts / a.groups;
-    Key mine = 0;                                  // lane g: the score of group g
-    for (int g = 0; g < a.groups; ++g) {
+    Key mine = 0;                                  // the score of group `group`
+    int group = lane;
+    if (p.lanes) {
+      // A group is p.lanes neighbouring lanes.
       Key b1 = 0, b2 = 0;
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
-        const int e = lane * NE + j - g * size;
-        if (e >= 0 && e < size) {
-          if (key[j] > b1) { b2 = b1; b1 = key[j]; }
-          else if (key[j] > b2) b2 = key[j];
+        b2 = larger(b2, smaller(b1, key[j]));
+        b1 = larger(b1, key[j]);
+      }
+      for (int o = 1; o < p.lanes; o <<= 1) {
+        const Key o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+        b2 = larger(smaller(b1, o1), larger(b2, o2));
+        b1 = larger(b1, o1);
+      }
+      group = lane / p.lanes;
+      mine = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+    } else {
+      for (int g = 0; g < a.groups; ++g) {
+        Key b1 = 0, b2 = 0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          const int e = lane * NE + j - g * size;
+          if (e >= 0 && e < size) {
+            b2 = larger(b2, smaller(b1, key[j]));
+            b1 = larger(b1, key[j]);
+          }
         }
+        const Key m1 = warp_max(b1);
+        Key score = m1;
+        if (a.top2) {
+          const int owner = __ffs(__ballot_sync(kAll, b1 == m1)) - 1;
+          score = key_of(value_of(m1) + value_of(warp_max(lane == owner ? b2 : b1)));
+        }
+        if (lane == g) mine = score;
       }
-      const Key m1 = warp_max(b1);
-      F score = value_of(m1);
-      if (a.top2) {
-        const int owner = __ffs(__ballot_sync(kAll, b1 == m1)) - 1;
-        score += value_of(warp_max(lane == owner ? b2 : b1));
-      }
-      if (lane == g) mine = key_of(score);
     }
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const Key other = __shfl_sync(kAll, mine, g);
-      rank += other > mine || (other == mine && g < lane) ? 1 : 0;
+      const Key other = __shfl_sync(kAll, mine, p.lanes ? g * p.lanes : g);
+      rank += other > mine || (other == mine && g < group) ? 1 : 0;
     }
-    const bool kept = lane < a.groups && rank < a.top_groups;
-    const unsigned keep = __ballot_sync(kAll, kept);
+    const bool kept = group < a.groups && rank < a.top_groups;
     if (check) {
       const F low = value_of(static_cast<Key>(~warp_max(kept ? static_cast<Key>(~mine) : Key(0))));
-      const F high = value_of(warp_max(lane < a.groups && !kept ? mine : Key(0)));
-      close = !(static_cast<float>(low - high) > 2.f * tau + 0x1p-20f * fabsf(static_cast<float>(low)));
+      const F high = value_of(warp_max(group < a.groups && !kept ? mine : Key(0)));
+      if (!(static_cast<float>(low - high) > 2.f * tau + 0x1p-20f * fabsf(static_cast<float>(low)))) close = 2;
     }
+    if (p.lanes) {
 #pragma unroll
-    for (int j = 0; j < NE; ++j)
-      if (!((keep >> ((lane * NE + j) / size & 31)) & 1u)) key[j] = 0;
-      else if (a.bias == nullptr && key[j] != 0) key[j] = key_of(static_cast<F>(l[j]));
+      for (int j = 0; j < NE; ++j)
+        if (!kept) key[j] = 0;
+    } else {
+      const unsigned keep = __ballot_sync(kAll, kept);
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (!((keep >> ((lane * NE + j) / size & 31)) & 1u)) key[j] = 0;
+    }
+    if (by_logit) {
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (key[j] != 0) key[j] = key_of(static_cast<F>(l[j]));
+    }
   }
   check = check && a.bias != nullptr;
 
+  if (kSorted) sort_lane<Key, NE>(key, num);
+  uint32_t numbers = 0;                            // four bits each, the head's lowest
+  if (kSorted)
+#pragma unroll
+    for (int j = 0; j < NE; ++j) numbers |= num[j] << (4 * j);
   Key best = 0;
 #pragma unroll
-  for (int j = 0; j < NE; ++j) best = key[j] > best ? key[j] : best;
-  int mine = -1;
-  F score = 0;
-  float my_l = 0.f, my_b = 0.f;
+  for (int j = 0; j < NE; ++j) best = larger(best, key[j]);
+  Key won = 0;                                     // lane i: the key of choice i
   const int rounds = a.top_k + (check ? 1 : 0);
   for (int i = 0; i < rounds; ++i) {
     const Key m = warp_max(best);
-    if (m == 0) break;                             // only the runner-up can be missing
-    const int owner = __ffs(__ballot_sync(kAll, best == m)) - 1;
-    int e = 0;
-    float el = 0.f, eb = 0.f;
-    if (lane == owner) {
-      bool found = false;
-      best = 0;
+    if (lane == i) won = m;
+    if (lane == __ffs(__ballot_sync(kAll, best == m)) - 1) {
+      if constexpr (kSorted) {
+        picked[i] = static_cast<uint16_t>(lane * NE + (numbers & 15u));
+        numbers >>= 4;
 #pragma unroll
-      for (int j = 0; j < NE; ++j) {
-        if (!found && key[j] == m) {
-          found = true;
-          key[j] = 0;
-          e = lane * NE + j;
-          el = l[j];
-          eb = bias[j];
+        for (int j = 0; j + 1 < NE; ++j) key[j] = key[j + 1];
+        key[NE - 1] = 0;
+        best = key[0];
+      } else {
+        int at = 0;
+#pragma unroll
+        for (int j = NE - 1; j >= 0; --j)
+          if (key[j] == m) at = j;
+        picked[i] = static_cast<uint16_t>(lane * NE + at);
+        best = 0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          if (j == at) key[j] = 0;
+          best = larger(best, key[j]);
         }
-        best = key[j] > best ? key[j] : best;
       }
     }
-    e = __shfl_sync(kAll, e, owner);
-    if (check) {
-      el = __shfl_sync(kAll, el, owner);
-      eb = __shfl_sync(kAll, eb, owner);
-    }
-    if (lane == i) { mine = e; score = value_of(m); my_l = el; my_b = eb; }
   }
+  __syncwarp();
   if (check) {
-    const int next = __shfl_down_sync(kAll, mine, 1);
-    const F below = __shfl_down_sync(kAll, score, 1);
-    const float l1 = __shfl_down_sync(kAll, my_l, 1), b1 = __shfl_down_sync(kAll, my_b, 1);
-    if (lane < a.top_k && next >= 0 && !(l1 == my_l && b1 == my_b))
-      close |= !(static_cast<float>(score - below) > tau + 0x1p-21f * fabsf(static_cast<float>(score)));
+    const Key below = __shfl_down_sync(kAll, won, 1);
+    if (lane < a.top_k && below != 0) {            // no runner-up: nothing to compare
+      const float score = static_cast<float>(value_of(won));
+      if (!(score - static_cast<float>(value_of(below)) > tau + 0x1p-21f * fabsf(score))) close |= 1;
+    }
   }
-  *near = __any_sync(kAll, close);
-  return lane < a.top_k ? mine : -1;
+  return close;
 }
 
 // The same choice from scores in 64 bits.
 template <int NE>
-__device__ __noinline__ int choose_wide(const RouteArgs& a, const float (&l)[NE], const float (&bias)[NE]) {
-  const int lane = threadIdx.x & 31;
+__device__ __noinline__ void choose_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+  const RouteArgs& a = p.a;
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < NE; ++j) top = fmaxf(top, l[j]);
@@ -194,148 +277,120 @@ __device__ __noinline__ int choose_wide(const RouteArgs& a, const float (&l)[NE]
     if (!a.sigmoid && total > 0) s[j] /= total;
     s[j] = l[j] == -INFINITY || bias[j] == -INFINITY ? -INFINITY : s[j] + static_cast<double>(bias[j]);
   }
-  bool near;
-  return choose<double, NE>(a, s, 0.f, false, l, bias, &near);
+  choose<double, NE>(p, s, 0.f, false, l, picked);
 }
 
-// Row of a token: cleaned logits, -infinity beyond the last expert.
+// Whether all that is close is a pair of choices with equal logits and equal biases, which no arithmetic can part.
+template <typename T>
+__device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, const uint16_t* picked) {
+  const RouteArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  float l = 0.f, b = 0.f;
+  if (a.bias != nullptr && lane <= a.top_k && lane < a.experts) {
+    const int e = min(static_cast<int>(picked[lane]), a.experts - 1);
+    l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
+    b = a.bias[e];
+  }
+  const float l1 = __shfl_down_sync(kAll, l, 1), b1 = __shfl_down_sync(kAll, b, 1);
+  return !__any_sync(kAll, (close & 2) || ((close & 1) && !(l == l1 && b == b1)));
+}
+
+// A lane's share of a row as it lies in memory.
+template <typename T, int NE> struct alignas(NE * sizeof(T) > 16 ? 16 : NE * sizeof(T)) Share { T v[NE]; };
+
 template <typename T, int NE>
-__device__ __forceinline__ void load_row(const RouteArgs& a, int64_t t, float (&l)[NE]) {
+__device__ __forceinline__ void load_share(const RouteParams& p, int64_t t, Share<T, NE>* to) {
+  const RouteArgs& a = p.a;
   const T* row = static_cast<const T*>(a.logits) + t * a.ld;
   const int e0 = (threadIdx.x & 31) * NE;
+  if (p.vec) {
+    if (e0 < a.experts) *to = *reinterpret_cast<const Share<T, NE>*>(row + e0);
+  } else {
 #pragma unroll
-  for (int j = 0; j < NE; ++j) {
-    const float v = to_f32<T>(row[min(e0 + j, a.experts - 1)]);
-    l[j] = e0 + j < a.experts ? clean(v) : -INFINITY;
+    for (int j = 0; j < NE; ++j) to->v[j] = row[min(e0 + j, a.experts - 1)];
   }
 }
-
-__device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
+// Cleaned logits, -infinity beyond the last expert.
+template <typename T, int NE>
+__device__ __forceinline__ void clean_share(const RouteArgs& a, const Share<T, NE>& from, float (&l)[NE]) {
+  const int e0 = (threadIdx.x & 31) * NE;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) l[j] = e0 + j < a.experts ? clean(to_f32<T>(from.v[j])) : -INFINITY;
+}
 
 // Shares of the choices among themselves, sum 1 (0 where every chosen logit is -infinity).  Scaled by the
 // largest so that it holds where the scores themselves would underflow: softmax(l) over the choices, or
 // sigmoid(l) / exp(m) with m = min(0, max l).
+__device__ __forceinline__ float share_size(bool sigmoid_scores, float l, float top) {
+  if (l == -INFINITY) return 0.f;
+  if (!sigmoid_scores) return expf(l - top);
+  return l > 0.f ? sigmoid(l) : expf(l - fminf(top, 0.f)) / (1.f + expf(l));
+}
 __device__ __forceinline__ float share(const RouteArgs& a, float l) {
-  const int lane = threadIdx.x & 31;
-  const bool live = lane < a.top_k && l != -INFINITY;
-  const float top = warp_max(live ? l : -INFINITY);
+  if (static_cast<int>(threadIdx.x & 31) >= a.top_k) l = -INFINITY;
+  const float top = warp_max(l);
   if (top == -INFINITY) return 0.f;
-  float q;
-  if (a.sigmoid) {
-    q = l > 0.f ? sigmoid(l) : expf(l - fminf(top, 0.f)) / (1.f + expf(l));
-  } else {
-    q = expf(l - top);
-  }
-  if (!live) q = 0.f;
+  const float q = share_size(a.sigmoid, l, top);
   return q / warp_sum(q);
 }
 
-template <typename T, int NE>
-__global__ void __launch_bounds__(kThreads) route_topk_kernel(const RouteParams p) {
-  extern __shared__ uint32_t smem[];
-  const RouteArgs& a = p.a;
-  uint32_t* bits = smem;                                             // [experts][words]
-  uint16_t* chosen = reinterpret_cast<uint16_t*>(bits + a.experts * p.words);   // [tokens_per_block][top_k]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x * p.tokens_per_block;
-  const int count = min(p.tokens_per_block, a.tokens - first);
-  for (int i = threadIdx.x; i < a.experts * p.words; i += kThreads) bits[i] = 0;
-
-  float bias[NE];
+// ---- rows in expert order --------------------------------------------------------------------------------------
+// Exclusive sums of value[0 .. n - 1] in place (n <= kMaxExperts), the total in `part[32]`, by the whole block.
+__device__ __forceinline__ void block_scan(int32_t* value, int n, int32_t* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int run = 0;
+  for (int e0 = 0; e0 < n; e0 += static_cast<int>(blockDim.x)) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    const int mine = e < n ? value[e] : 0;
+    int sum = mine;
 #pragma unroll
-  for (int j = 0; j < NE; ++j) {
-    const int e = min(lane * NE + j, a.experts - 1);
-    bias[j] = a.bias ? clean(a.bias[e]) : 0.f;
-  }
-  const bool scored = a.bias != nullptr || (a.top2 && a.top_groups < a.groups);   // the order needs the scores
-  __syncthreads();
-
-  for (int i = warp; i < count; i += kWarps) {
-    const int64_t t = first + i;
-    int e = -1;
-    float w = 0.f;
-    if (a.mask == nullptr || a.mask[t]) {
-      float l[NE];
-      load_row<T, NE>(a, t, l);
-      float top = 0.f, total = 1.f;
-      float s[NE];
-#pragma unroll
-      for (int j = 0; j < NE; ++j) s[j] = l[j];
-      if (!a.sigmoid && (scored || !a.renormalise)) {
-        top = l[0];
-#pragma unroll
-        for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
-        top = warp_max(top);
-        total = 0.f;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          s[j] = l[j] == -INFINITY ? 0.f : expf(l[j] - top);
-          total += s[j];
-        }
-        total = warp_sum(total);
-      }
-      bool near = false;
-      if (scored) {
-        const float inv = total > 0.f ? 1.f / total : 0.f;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          const float prob = a.sigmoid ? sigmoid(l[j]) : s[j] * inv;
-          s[j] = l[j] == -INFINITY || bias[j] == -INFINITY ? -INFINITY : prob + bias[j];
-        }
-        // Error of one score: exp 2^-22, sum (NE + 5) 2^-24 + 2^-22, quotient and product 2^-23, each of the
-        // row's largest probability 1 / total; twice that for a difference.  Sigmoid: 1.5 * 2^-22 of at most 1.
-        const float tau = a.sigmoid ? 0x1p-20f : (NE + 18) * 0x1p-23f * inv;
-        e = choose<float, NE>(a, s, tau, true, l, bias, &near);
-        if (near) e = choose_wide<NE>(a, l, bias);
-      } else {
-        e = choose<float, NE>(a, l, 0.f, false, l, bias, &near);
-      }
-      const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
-      if (a.renormalise) w = share(a, le);
-      else if (a.sigmoid) w = sigmoid(le);
-      else w = le == -INFINITY ? 0.f : expf(le - top) / total;
-      w *= a.scale;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kAll, sum, o);
+      if (lane >= o) sum += v;
     }
-    if (lane < a.top_k) {
-      a.idx[t * a.top_k + lane] = e;
-      a.weights[t * a.top_k + lane] = w;
-      chosen[i * a.top_k + lane] = static_cast<uint16_t>(e);           // 0xffff: none
-      if (e >= 0) atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
-    }
-  }
-  __syncthreads();
-
-  // Choices per expert: to the second kernel, or (one block) straight into the offsets.
-  __shared__ int32_t base[kMaxExperts + 1];
-  for (int e = threadIdx.x; e < a.experts; e += kThreads) {
-    int n = 0;
-    for (int w = 0; w < p.words; ++w) n += __popc(bits[e * p.words + w]);
-    if (gridDim.x > 1) p.counts[static_cast<int64_t>(blockIdx.x) * a.experts + e] = static_cast<uint16_t>(n);
-    base[e] = gridDim.x > 1 ? 0 : n;
-  }
-  __syncthreads();
-  if (gridDim.x == 1) {
+    if (lane == 31) part[warp] = sum;
+    __syncthreads();
     if (warp == 0) {
-      int run = 0;
-      for (int e0 = 0; e0 < a.experts; e0 += 32) {
-        const int n = e0 + lane < a.experts ? base[e0 + lane] : 0;
-        int sum = n;
+      const int own = lane < warps ? part[lane] : 0;
+      int all = own;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(kAll, sum, o);
-          if (lane >= o) sum += v;
-        }
-        if (e0 + lane < a.experts) {
-          base[e0 + lane] = run + sum - n;
-          a.offsets[e0 + lane] = run + sum - n;
-        }
-        run += __shfl_sync(kAll, sum, 31);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kAll, all, o);
+        if (lane >= o) all += v;
       }
-      if (lane == 0) a.offsets[a.experts] = run;
+      part[lane] = all - own;
+      if (lane == 31) part[32] = all;
     }
     __syncthreads();
+    if (e < n) value[e] = run + part[warp] + sum - mine;
+    run += part[32];
+    __syncthreads();
   }
-  for (int i = threadIdx.x; i < count * a.top_k; i += kThreads) {
+  if (threadIdx.x == 0) part[32] = run;
+  __syncthreads();
+}
+
+// Counts and ranks of the block's marked choices.  With one block the rows are final; otherwise the counts go to
+// the second kernel, and the rows start at zero for every expert.
+__device__ __forceinline__ void finish_block(const RouteParams& p, const uint32_t* bits, const uint16_t* chosen,
+                                             int first, int count) {
+  __shared__ int32_t base[kMaxExperts];
+  __shared__ int32_t part[33];
+  const RouteArgs& a = p.a;
+  const bool alone = gridDim.x == 1;
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+    int n = 0;
+    for (int w = 0; w < p.words; ++w) n += __popc(bits[e * p.words + w]);
+    if (!alone) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + e] = static_cast<uint16_t>(n);
+    base[e] = alone ? n : 0;
+  }
+  if (!alone && threadIdx.x == 0 && (a.experts & 1)) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + a.experts] = 0;
+  __syncthreads();
+  if (alone) {
+    block_scan(base, a.experts, part);
+    for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) a.offsets[e] = e < a.experts ? base[e] : part[32];
+  }
+  for (int i = threadIdx.x; i < count * a.top_k; i += blockDim.x) {
     const int e = chosen[i], tok = i / a.top_k;
     int row = -1;
     if (e != 0xffff) {
@@ -347,107 +402,494 @@ __global__ void __launch_bounds__(kThreads) route_topk_kernel(const RouteParams 
   }
 }
 
-// Adds to every choice the rows of earlier experts and of earlier blocks of its own expert.
-__global__ void __launch_bounds__(kThreads) route_rows_kernel(const RouteParams p) {
+template <typename T, int NE, int kMost>
+__global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams p) {
+  extern __shared__ uint32_t smem[];
+  __shared__ uint16_t picks[kMost / 32][32];
   const RouteArgs& a = p.a;
-  __shared__ int32_t before[kMaxExperts], total[kMaxExperts];
-  const int lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < a.experts; e += kThreads) {
-    int sum = 0, mine = 0;
-    for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-      if (b == static_cast<int>(blockIdx.x)) mine = sum;
-      sum += p.counts[static_cast<int64_t>(b) * a.experts + e];
-    }
-    before[e] = mine;
-    total[e] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int run = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int n = e0 + lane < a.experts ? total[e0 + lane] : 0;
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kAll, sum, o);
-        if (lane >= o) sum += v;
-      }
-      if (e0 + lane < a.experts) {
-        before[e0 + lane] += run + sum - n;
-        if (blockIdx.x == 0) a.offsets[e0 + lane] = run + sum - n;
-      }
-      run += __shfl_sync(kAll, sum, 31);
-    }
-    if (blockIdx.x == 0 && lane == 0) a.offsets[a.experts] = run;
-  }
-  __syncthreads();
+  uint32_t* bits = smem;                                             // [experts][words]
+  uint16_t* chosen = reinterpret_cast<uint16_t*>(bits + a.experts * p.words);   // [tokens_per_block][top_k]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int first = blockIdx.x * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
-  for (int i = threadIdx.x; i < count * a.top_k; i += kThreads) {
+  uint16_t* const picked = picks[warp];
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  Share<T, NE> next{};
+  if (warp < count) load_share<T, NE>(p, first + warp, &next);
+  float bias[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) bias[j] = a.bias ? clean(a.bias[min(lane * NE + j, a.experts - 1)]) : 0.f;
+  for (int i = threadIdx.x; i < a.experts * p.words; i += blockDim.x) bits[i] = 0;
+  const bool grouped_sum = a.top2 && a.top_groups < a.groups;
+  const bool scored = a.bias != nullptr || grouped_sum;              // the order needs the scores
+  __syncthreads();
+
+  for (int i = warp; i < count; i += warps) {
+    const int64_t t = first + i;
+    const Share<T, NE> raw = next;
+    if (i + warps < count) load_share<T, NE>(p, t + warps, &next);
+    int e = -1;
+    float w = 0.f;
+    if (a.mask == nullptr || a.mask[t]) {
+      float l[NE], s[NE];
+      clean_share<T, NE>(a, raw, l);
+      float top = 0.f, total = 1.f;
+#pragma unroll
+      for (int j = 0; j < NE; ++j) s[j] = l[j];
+      if (!a.sigmoid && (scored || !a.renormalise)) {
+        top = l[0];
+#pragma unroll
+        for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
+        top = warp_max(top);
+        total = 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          // The weights are made of these where they are not renormalised: then to the full 2^-22.
+          const float x = a.renormalise ? __expf(l[j] - top) : expf(l[j] - top);
+          s[j] = l[j] == -INFINITY ? 0.f : x;
+          total += s[j];
+        }
+        total = warp_sum(total);
+      }
+      if (scored) {
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          const float prob = a.sigmoid ? quick_sigmoid(l[j]) : s[j] * inv;
+          s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
+        }
+        const int close = choose<float, NE>(p, s, score_error(a.sigmoid, NE, inv), true, l, picked);
+        if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, picked)) choose_wide<NE>(p, l, bias, picked);
+      } else {
+        choose<float, NE>(p, l, 0.f, false, l, picked);
+      }
+      e = lane < a.top_k ? picked[lane] : -1;
+      const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
+      if (a.renormalise) w = share(a, le);
+      else if (a.sigmoid) w = sigmoid(le);
+      else w = le == -INFINITY ? 0.f : expf(le - top) / total;
+      w *= a.scale;
+      __syncwarp();                                                  // picked is read
+    }
+    if (lane < a.top_k) {
+      a.idx[t * a.top_k + lane] = e;
+      a.weights[t * a.top_k + lane] = w;
+      chosen[i * a.top_k + lane] = static_cast<uint16_t>(e);           // 0xffff: none
+      if (e >= 0) atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
+    }
+  }
+  __syncthreads();
+  finish_block(p, bits, chosen, first, count);
+}
+
+// ---- a thread per token ----------------------------------------------------------------------------------------
+// choose() by one thread over all experts; numbers go to picked[0 .. top_k - 1].  Returns whether the choice has to be
+// repeated in 64 bits.
+template <typename F, int NE>
+__device__ __forceinline__ bool choose_alone(const RouteParams& p, const F (&s)[NE], float tau, bool check,
+                                             const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+  using Key = decltype(key_of(F()));
+  const RouteArgs& a = p.a;
+  Key key[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) key[j] = j < a.experts ? key_of(s[j]) : Key(0);
+  bool close = false;
+  if (a.top_groups < a.groups) {
+    const int size = a.experts / a.groups;
+    Key score[NE];                                 // of the group of each expert
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      Key b1 = 0, b2 = 0;
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i / size == j / size) {
+          b2 = larger(b2, smaller(b1, key[i]));
+          b1 = larger(b1, key[i]);
+        }
+      score[j] = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+    }
+    Key low = ~Key(0), high = 0;
+    unsigned keep = 0;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      if (j >= a.experts) continue;
+      int rank = 0;
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i < a.experts && i % size == 0) rank += score[i] > score[j] || (score[i] == score[j] && i / size < j / size) ? 1 : 0;
+      if (rank < a.top_groups) {
+        keep |= 1u << j;
+        low = smaller(low, score[j]);
+      } else {
+        high = larger(high, score[j]);
+      }
+    }
+    if (check) {
+      const float a0 = static_cast<float>(value_of(low)), gap = static_cast<float>(value_of(low) - value_of(high));
+      close = !(gap > 2.f * tau + 0x1p-20f * fabsf(a0));
+    }
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      if (!((keep >> j) & 1u)) key[j] = 0;
+      else if (a.bias == nullptr) key[j] = key_of(static_cast<F>(l[j]));
+    }
+  }
+  check = check && a.bias != nullptr;
+  const int rounds = a.top_k + (check ? 1 : 0);
+  Key before = 0;
+  float l0 = 0.f, b0 = 0.f;
+  for (int i = 0; i < rounds; ++i) {
+    Key best = 0;
+    int at = 0;
+    float l1 = 0.f, b1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+      if (key[j] > best) {
+        best = key[j];
+        at = j;
+        l1 = l[j];
+        b1 = bias[j];
+      }
+    if (best == 0) break;                          // only the runner-up can be missing
+    if (check && i > 0 && !(l0 == l1 && b0 == b1)) {
+      const float a0 = static_cast<float>(value_of(before));
+      close |= !(a0 - static_cast<float>(value_of(best)) > tau + 0x1p-21f * fabsf(a0));
+    }
+    if (i < a.top_k) picked[i] = static_cast<uint16_t>(at);
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+      if (j == at) key[j] = 0;
+    before = best;
+    l0 = l1;
+    b0 = b1;
+  }
+  return close;
+}
+template <int NE>
+__device__ __noinline__ void choose_alone_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+  const RouteArgs& a = p.a;
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) top = fmaxf(top, l[j]);
+  double s[NE], total = 0;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    const double v = static_cast<double>(l[j]);
+    s[j] = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : (l[j] == -INFINITY ? 0.0 : exp(v - static_cast<double>(top)));
+    total += s[j];
+  }
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    if (!a.sigmoid && total > 0) s[j] /= total;
+    s[j] = l[j] == -INFINITY || bias[j] == -INFINITY ? -INFINITY : s[j] + static_cast<double>(bias[j]);
+  }
+  choose_alone<double, NE>(p, s, 0.f, false, l, bias, picked);
+}
+
+template <typename T, int NE>
+__device__ __forceinline__ void load_token(const RouteParams& p, int64_t t, float (&l)[NE]) {
+  const RouteArgs& a = p.a;
+  const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+  if (p.vec) {
+    const Share<T, NE> raw = *reinterpret_cast<const Share<T, NE>*>(row);
+#pragma unroll
+    for (int j = 0; j < NE; ++j) l[j] = clean(to_f32<T>(raw.v[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < NE; ++j) l[j] = j < a.experts ? clean(to_f32<T>(row[j])) : -INFINITY;
+  }
+}
+
+template <typename T, int NE>
+__global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const RouteParams p) {
+  extern __shared__ uint32_t smem[];
+  const RouteArgs& a = p.a;
+  uint32_t* bits = smem;                                             // [experts][words]
+  uint16_t* chosen = reinterpret_cast<uint16_t*>(bits + a.experts * p.words);   // [tokens_per_block][top_k]
+  const int first = blockIdx.x * p.tokens_per_block;
+  const int count = min(p.tokens_per_block, a.tokens - first);
+  asm volatile("griddepcontrol.launch_dependents;");
+  for (int i = threadIdx.x; i < a.experts * p.words; i += blockDim.x) bits[i] = 0;
+  const bool scored = a.bias != nullptr || (a.top2 && a.top_groups < a.groups);
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int64_t t = first + i;
+    const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+    uint16_t* const picked = chosen + i * a.top_k;
+    const bool live = a.mask == nullptr || a.mask[t];
+    float top = 0.f, total = 1.f;
+    if (live) {
+      float l[NE], s[NE], bias[NE];
+      load_token<T, NE>(p, t, l);
+#pragma unroll
+      for (int j = 0; j < NE; ++j) {
+        bias[j] = a.bias ? clean(a.bias[min(j, a.experts - 1)]) : 0.f;
+        s[j] = l[j];
+      }
+      if (!a.sigmoid && (scored || !a.renormalise)) {
+        top = l[0];
+#pragma unroll
+        for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
+        total = 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          s[j] = l[j] == -INFINITY ? 0.f : expf(l[j] - top);
+          total += s[j];
+        }
+      }
+      if (scored) {
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          const float prob = a.sigmoid ? quick_sigmoid(l[j]) : s[j] * inv;
+          s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
+        }
+        if (choose_alone<float, NE>(p, s, score_error(a.sigmoid, NE, inv), true, l, bias, picked))
+          choose_alone_wide<NE>(p, l, bias, picked);
+      } else {
+        choose_alone<float, NE>(p, l, 0.f, false, l, bias, picked);
+      }
+    }
+    float best = -INFINITY, sum = 0.f;
+    if (live && a.renormalise) {
+      for (int k = 0; k < a.top_k; ++k) best = fmaxf(best, clean(to_f32<T>(row[picked[k]])));
+      for (int k = 0; k < a.top_k; ++k) sum += share_size(a.sigmoid, clean(to_f32<T>(row[picked[k]])), best);
+    }
+    for (int k = 0; k < a.top_k; ++k) {
+      int e = -1;
+      float w = 0.f;
+      if (live) {
+        e = picked[k];
+        const float le = clean(to_f32<T>(row[e]));
+        if (a.renormalise) w = sum > 0.f ? share_size(a.sigmoid, le, best) / sum : 0.f;
+        else if (a.sigmoid) w = sigmoid(le);
+        else w = le == -INFINITY ? 0.f : expf(le - top) / total;
+        w *= a.scale;
+        atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
+      } else {
+        picked[k] = 0xffff;
+      }
+      a.idx[t * a.top_k + k] = e;
+      a.weights[t * a.top_k + k] = w;
+    }
+  }
+  __syncthreads();
+  finish_block(p, bits, chosen, first, count);
+}
+
+// Adds to every choice the rows of earlier experts and of earlier blocks of its own expert.  A thread sums two
+// neighbouring experts over a strip of the blocks; whole numbers, so the order of the additions is free.
+__global__ void __launch_bounds__(kMostThreads, 1) route_rows_kernel(const RouteParams p) {
+  const RouteArgs& a = p.a;
+  __shared__ int32_t before[kMaxExperts + 1], total[kMaxExperts + 1], part[33];
+  for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) before[e] = total[e] = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int pairs = p.pitch / 2, me = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
+  int width = 1;                                   // threads abreast: a power of two
+  while (width < pairs) width <<= 1;
+  const int strips = static_cast<int>(blockDim.x) / width, strip = threadIdx.x / width, col = threadIdx.x % width;
+  const uint32_t* counts = reinterpret_cast<const uint32_t*>(p.counts);
+  int b0 = 0, b1 = 0, t0 = 0, t1 = 0;
+  if (col < pairs) {
+#pragma unroll 8
+    for (int b = strip; b < blocks; b += strips) {
+      const uint32_t c = counts[static_cast<int64_t>(b) * pairs + col];
+      const int lo = c & 0xffffu, hi = c >> 16;
+      t0 += lo;
+      t1 += hi;
+      b0 += b < me ? lo : 0;
+      b1 += b < me ? hi : 0;
+    }
+  }
+  for (int o = width; o < 32; o <<= 1) {           // lanes of the same column
+    b0 += __shfl_xor_sync(kAll, b0, o);
+    b1 += __shfl_xor_sync(kAll, b1, o);
+    t0 += __shfl_xor_sync(kAll, t0, o);
+    t1 += __shfl_xor_sync(kAll, t1, o);
+  }
+  if (col < pairs && (threadIdx.x & 31) < static_cast<unsigned>(width)) {
+    atomicAdd(before + 2 * col, b0);
+    atomicAdd(before + 2 * col + 1, b1);
+    atomicAdd(total + 2 * col, t0);
+    atomicAdd(total + 2 * col + 1, t1);
+  }
+  __syncthreads();
+  block_scan(total, a.experts, part);
+  if (me == 0)
+    for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) a.offsets[e] = e < a.experts ? total[e] : part[32];
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) before[e] += total[e];
+  __syncthreads();
+  const int first = me * p.tokens_per_block;
+  const int count = min(p.tokens_per_block, a.tokens - first);
+  for (int i = threadIdx.x; i < count * a.top_k; i += blockDim.x) {
     const int64_t at = static_cast<int64_t>(first) * a.top_k + i;
     const int e = a.idx[at];
     if (e >= 0) a.rows[at] += before[e];
   }
 }
 
+// ---- gradient --------------------------------------------------------------------------------------------------
 // dl from dw, idx constant.  With c = scale and a_k the shares of the choices (renormalised):
 //   softmax  dl_k = c a_k (g_k - <g, a>)                 sigmoid  the same times (1 - p_k)
 // else softmax  dl_e = c p_e (g_e - <g, p>)              sigmoid  dl_k = c g_k p_k (1 - p_k).
+// All but the third leave the experts that were not chosen at zero: a row of zeros is stored and the choices over it.
 template <typename T, int NE>
-__global__ void __launch_bounds__(kThreads) route_topk_backward_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(256) route_warp_backward_kernel(const RouteParams p) {
   const RouteArgs& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp; t < a.tokens;
-       t += static_cast<int64_t>(gridDim.x) * kWarps) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+  const bool whole = !a.renormalise && !a.sigmoid;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < a.tokens; t += warps) {
     int e = lane < a.top_k ? a.idx[t * a.top_k + lane] : -1;
     if (e >= a.experts) e = -1;
     const float g = e >= 0 ? p.dweights[t * a.top_k + lane] : 0.f;
     const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
-    float d, rest = 0.f, top = 0.f, inv = 0.f;
-    float l[NE];
-    if (a.renormalise) {
-      const float q = share(a, le);
-      d = a.scale * q * (g - warp_sum(g * q));
-      if (a.sigmoid) d *= sigmoid(-le);
-    } else if (a.sigmoid) {
-      d = a.scale * g * sigmoid(le) * sigmoid(-le);
-    } else {
-      load_row<T, NE>(a, t, l);
-      top = l[0];
-#pragma unroll
-      for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
-      top = warp_max(top);
-      float total = 0.f;
-#pragma unroll
-      for (int j = 0; j < NE; ++j) total += l[j] == -INFINITY ? 0.f : expf(l[j] - top);
-      total = warp_sum(total);
-      inv = total > 0.f ? 1.f / total : 0.f;
-      const float prob = le == -INFINITY ? 0.f : expf(le - top) * inv;
-      rest = warp_sum(g * prob);
-      d = g;
-    }
-    if (le == -INFINITY) d = 0.f;
-    float out[NE];
-#pragma unroll
-    for (int j = 0; j < NE; ++j) out[j] = 0.f;
-    for (int k = 0; k < a.top_k; ++k) {
-      const int ek = __shfl_sync(kAll, e, k);
-      const float dk = __shfl_sync(kAll, d, k);
-#pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (ek == lane * NE + j) out[j] = dk;
-    }
-    if (!a.renormalise && !a.sigmoid) {
-      const bool any = __any_sync(kAll, e >= 0);
-#pragma unroll
-      for (int j = 0; j < NE; ++j)
-        out[j] = any && l[j] != -INFINITY ? a.scale * expf(l[j] - top) * inv * (out[j] - rest) : 0.f;
-    }
     T* row = static_cast<T*>(p.dlogits) + t * a.experts;
+    if (!whole) {
+      const Share<T, NE> zero{};
+      const int e0 = lane * NE;
+      if (p.vec) {
+        if (e0 < a.experts) *reinterpret_cast<Share<T, NE>*>(row + e0) = zero;
+      } else {
+        for (int j = lane; j < a.experts; j += 32) row[j] = from_f32<T>(0.f);
+      }
+      float d;
+      if (a.renormalise) {
+        const float q = share(a, le);
+        d = a.scale * q * (g - warp_sum(g * q));
+        if (a.sigmoid) d *= sigmoid(-le);
+      } else {
+        d = a.scale * g * sigmoid(le) * sigmoid(-le);
+      }
+      __syncwarp();                                // the zeros come first
+      if (e >= 0 && le != -INFINITY) row[e] = from_f32<T>(d);
+      continue;
+    }
+    Share<T, NE> raw;
+    load_share<T, NE>(p, t, &raw);
+    float l[NE];
+    clean_share<T, NE>(a, raw, l);
+    float top = l[0], total = 0.f;
+#pragma unroll
+    for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
+    top = warp_max(top);
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      l[j] = l[j] == -INFINITY ? 0.f : expf(l[j] - top);
+      total += l[j];
+    }
+    total = warp_sum(total);
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float prob = le == -INFINITY ? 0.f : expf(le - top) * inv;
+    const float rest = warp_sum(g * prob);
+    const bool any = __any_sync(kAll, e >= 0);     // a masked token has no gradient
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      l[j] = any ? -a.scale * l[j] * inv * rest : 0.f;
+      raw.v[j] = from_f32<T>(l[j]);
+    }
+    if (p.vec) {
+      if (lane * NE < a.experts) *reinterpret_cast<Share<T, NE>*>(row + lane * NE) = raw;
+    } else {
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (lane * NE + j < a.experts) row[lane * NE + j] = raw.v[j];
+    }
+    __syncwarp();
+    if (e >= 0) row[e] = from_f32<T>(a.scale * prob * (g - rest));
+  }
+}
+
+template <typename T, int NE>
+__global__ void __launch_bounds__(128) route_thread_backward_kernel(const RouteParams p) {
+  const RouteArgs& a = p.a;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
+  if (t >= a.tokens) return;
+  const int32_t* idx = a.idx + t * a.top_k;
+  const float* g = p.dweights + t * a.top_k;
+  float l[NE], d[NE];
+  load_token<T, NE>(p, t, l);
+  unsigned picked = 0;                             // experts that were chosen
+#pragma unroll
+  for (int j = 0; j < NE; ++j) d[j] = 0.f;
+  for (int k = 0; k < a.top_k; ++k) {
+    const int e = idx[k];
+    const float gk = g[k];
+    if (e < 0 || e >= a.experts) continue;
+    picked |= 1u << e;
 #pragma unroll
     for (int j = 0; j < NE; ++j)
-      if (lane * NE + j < a.experts) row[lane * NE + j] = from_f32<T>(out[j]);
+      if (j == e) d[j] = gk;                       // g by expert
   }
+  const bool whole = !a.renormalise && !a.sigmoid;
+  if (a.renormalise || whole) {
+    // Shares of the choices (or, whole, of all experts), then c a (g - <g, a>).
+    float top = -INFINITY, total = 0.f, rest = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+      if (whole || ((picked >> j) & 1u)) top = fmaxf(top, l[j]);
+    float q[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      q[j] = picked && (whole || ((picked >> j) & 1u)) ? share_size(a.sigmoid, l[j], top) : 0.f;
+      total += q[j];
+      rest = fmaf(q[j], d[j], rest);
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      d[j] = a.scale * q[j] * inv * (d[j] - rest * inv);
+      if (a.sigmoid) d[j] *= sigmoid(-l[j]);
+      if (q[j] == 0.f) d[j] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NE; ++j) d[j] = l[j] == -INFINITY ? 0.f : a.scale * d[j] * sigmoid(l[j]) * sigmoid(-l[j]);
+  }
+  T* row = static_cast<T*>(p.dlogits) + t * a.experts;
+  Share<T, NE> out;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) out.v[j] = from_f32<T>(d[j]);
+  if (p.vec) {
+    *reinterpret_cast<Share<T, NE>*>(row) = out;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NE; ++j)
+      if (j < a.experts) row[j] = out.v[j];
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------
+constexpr size_t kMaxRouteSmem = 96 * 1024;
+
+size_t route_smem(int experts, int top_k, int tokens_per_block) {
+  return static_cast<size_t>(experts) * (tokens_per_block / 32) * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2;
+}
+
+// Experts of a lane (or of a thread) that the kernels are compiled for.
+int share_of(int experts) {
+  if (experts <= kThreadExperts) return experts <= 4 ? 4 : 8;
+  int ne = 1;
+  while (ne * 32 < experts) ne *= 2;
+  return ne;
+}
+
+// Few tokens stay in one block, which needs no second kernel; more get about a block per SM.
+int tokens_per_block(int tokens, int experts, int top_k) {
+  int tpb;
+  if (experts <= kThreadExperts) {
+    tpb = tokens <= 1024 ? tokens : (tokens + 591) / 592;
+    if (tpb < 128 && tokens > 1024) tpb = 128;
+    if (tpb > 1024) tpb = 1024;
+  } else {
+    tpb = tokens <= 96 ? tokens : (tokens + 147) / 148;
+  }
+  tpb = (tpb + 31) / 32 * 32;
+  if (tpb < 32) tpb = 32;
+  while (tpb > 32 && route_smem(experts, top_k, tpb) > kMaxRouteSmem) tpb -= 32;
+  return tpb;
 }
 
 int sm_count() {
@@ -457,44 +899,50 @@ int sm_count() {
   return sms;
 }
 
-constexpr int kMinTokensPerBlock = 32;
-constexpr size_t kMaxRouteSmem = 96 * 1024;
-
-size_t route_smem(int experts, int top_k, int tokens_per_block) {
-  return static_cast<size_t>(experts) * (tokens_per_block / 32) * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2;
-}
-
-// A block per SM, as many tokens as its bit marks have room for.
-int tokens_per_block(int tokens, int experts, int top_k) {
-  const int sms = 148;
-  int tpb = (tokens + sms - 1) / sms;
-  tpb = (tpb + 31) / 32 * 32;
-  if (tpb < kMinTokensPerBlock) tpb = kMinTokensPerBlock;
-  while (tpb > 32 && route_smem(experts, top_k, tpb) > kMaxRouteSmem) tpb -= 32;
-  return tpb;
+template <class Kernel> void launch_route(Kernel kernel, const RouteParams& p, int blocks, int threads, size_t smem, cudaStream_t stream) {
+  if (smem > 32 * 1024)
+    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  kernel<<<blocks, threads, smem, stream>>>(p);
 }
 
 template <typename T, int NE>
-void launch_route(const RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
+void launch_warps(const RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
   if (backward) {
-    route_topk_backward_kernel<T, NE><<<blocks, kThreads, 0, stream>>>(p);
+    const int64_t want = (static_cast<int64_t>(p.a.tokens) + 7) / 8, most = 8ll * sm_count();
+    route_warp_backward_kernel<T, NE><<<static_cast<int>(want < most ? want : most), 256, 0, stream>>>(p);
     return;
   }
-  if (smem > 40 * 1024)
-    PCCL_CUDA(cudaFuncSetAttribute(route_topk_kernel<T, NE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(smem)));
-  route_topk_kernel<T, NE><<<blocks, kThreads, smem, stream>>>(p);
+  constexpr int kMost = NE <= 8 ? 1024 : 512;      // 64 or 128 registers a thread
+  int threads = (p.a.tokens < p.tokens_per_block ? p.a.tokens : p.tokens_per_block) * 32;
+  threads = threads < 128 ? 128 : threads > kMost ? kMost : threads;
+  launch_route(route_warp_kernel<T, NE, kMost>, p, blocks, threads, smem, stream);
 }
 
-void launch_route_any(const RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
-  const int per_lane = (p.a.experts + 31) / 32;
-  PCCL_BLOCK_TYPES(p.a.dtype, T,
-    if (per_lane <= 1) launch_route<T, 1>(p, backward, blocks, smem, stream);
-    else if (per_lane <= 2) launch_route<T, 2>(p, backward, blocks, smem, stream);
-    else if (per_lane <= 4) launch_route<T, 4>(p, backward, blocks, smem, stream);
-    else if (per_lane <= 8) launch_route<T, 8>(p, backward, blocks, smem, stream);
-    else if (per_lane <= 16) launch_route<T, 16>(p, backward, blocks, smem, stream);
-    else launch_route<T, 32>(p, backward, blocks, smem, stream))
+template <typename T, int NE>
+void launch_threads(const RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
+  if (backward) route_thread_backward_kernel<T, NE><<<(p.a.tokens + 127) / 128, 128, 0, stream>>>(p);
+  else launch_route(route_thread_kernel<T, NE>, p, blocks, p.tokens_per_block < 128 ? 128 : p.tokens_per_block, smem, stream);
+}
+
+void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
+  const RouteArgs& a = p.a;
+  const int ne = share_of(a.experts), bytes = dtype_bytes(a.dtype);
+  const int piece = ne * bytes < 16 ? ne * bytes : 16;
+  const bool alone = a.experts <= kThreadExperts;
+  p.vec = (alone ? a.experts == ne : a.experts % ne == 0) && reinterpret_cast<uintptr_t>(a.logits) % piece == 0 &&
+          a.ld * bytes % piece == 0 &&
+          (!backward || (reinterpret_cast<uintptr_t>(p.dlogits) % piece == 0 && static_cast<int64_t>(a.experts) * bytes % piece == 0));
+  const int size = a.experts / a.groups;
+  p.lanes = size % ne == 0 && ((size / ne) & (size / ne - 1)) == 0 && size / ne <= 32 ? size / ne : 0;
+  PCCL_BLOCK_TYPES(a.dtype, T,
+    if (alone && ne == 4) launch_threads<T, 4>(p, backward, blocks, smem, stream);
+    else if (alone) launch_threads<T, 8>(p, backward, blocks, smem, stream);
+    else if (ne == 1) launch_warps<T, 1>(p, backward, blocks, smem, stream);
+    else if (ne == 2) launch_warps<T, 2>(p, backward, blocks, smem, stream);
+    else if (ne == 4) launch_warps<T, 4>(p, backward, blocks, smem, stream);
+    else if (ne == 8) launch_warps<T, 8>(p, backward, blocks, smem, stream);
+    else if (ne == 16) launch_warps<T, 16>(p, backward, blocks, smem, stream);
+    else launch_warps<T, 32>(p, backward, blocks, smem, stream))
   PCCL_CUDA(cudaGetLastError());
 }
 
@@ -503,7 +951,7 @@ void launch_route_any(const RouteParams& p, bool backward, int blocks, size_t sm
 size_t route_workspace(int tokens, int experts, int top_k) {
   const int tpb = tokens_per_block(tokens, experts, top_k);
   const int blocks = (tokens + tpb - 1) / tpb;
-  return blocks > 1 ? static_cast<size_t>(blocks) * experts * sizeof(uint16_t) : 0;
+  return blocks > 1 ? static_cast<size_t>(blocks) * ((experts + 1) / 2 * 2) * sizeof(uint16_t) : 0;
 }
 
 void route_topk(const RouteArgs& a, cudaStream_t stream) {
@@ -511,14 +959,24 @@ void route_topk(const RouteArgs& a, cudaStream_t stream) {
   p.a = a;
   p.tokens_per_block = tokens_per_block(a.tokens, a.experts, a.top_k);
   p.words = p.tokens_per_block / 32;
+  p.pitch = (a.experts + 1) / 2 * 2;
   int blocks = (a.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks < 1) blocks = 1;
   p.counts = static_cast<uint16_t*>(a.workspace);
   PCCL_CHECK(blocks == 1 || p.counts != nullptr, "route_topk: no workspace");
-  launch_route_any(p, false, blocks, route_smem(a.experts, a.top_k, p.tokens_per_block), stream);
+  launch_any(p, false, blocks, route_smem(a.experts, a.top_k, p.tokens_per_block), stream);
   if (blocks > 1) {
-    route_rows_kernel<<<blocks, kThreads, 0, stream>>>(p);
-    PCCL_CUDA(cudaGetLastError());
+    // Its blocks may start while the first kernel ends; they wait for its results on the device.
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(kMostThreads);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    PCCL_CUDA(cudaLaunchKernelEx(&config, route_rows_kernel, p));
   }
 }
 
@@ -528,8 +986,7 @@ void route_topk_backward(const RouteArgs& a, const float* dweights, void* dlogit
   p.a = a;
   p.dweights = dweights;
   p.dlogits = dlogits;
-  const int64_t want = (static_cast<int64_t>(a.tokens) + kWarps - 1) / kWarps, most = 4ll * sm_count();
-  launch_route_any(p, true, static_cast<int>(want < most ? want : most), 0, stream);
+  launch_any(p, true, 0, 0, stream);
 }
 
 }  // namespace block
