@@ -6,6 +6,7 @@
 // streams and graph captures need no care here.
 #include "block_bindings.h"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -93,6 +94,11 @@ void once(variable_list& grads) {
   for (size_t i = 0; i < at_index.size(); ++i) grads[at_index[i]] = out[i];
 }
 
+// Contiguous and uninitialised, on the device of `like`.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && wants_grad(*t); }
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
@@ -131,15 +137,14 @@ variable_list route_run(const RouteCall& c, const Tensor& logits, const OptTenso
   const Tensor m = mask.has_value() ? mask->contiguous() : Tensor();
   if (b.defined()) a.bias = b.const_data_ptr<float>();
   if (m.defined()) a.mask = reinterpret_cast<const uint8_t*>(m.const_data_ptr<bool>());
-  const auto ints = logits.options().dtype(at::kInt).requires_grad(false);
-  Tensor idx = at::empty({a.tokens, a.top_k}, ints);
-  Tensor weights = at::empty({a.tokens, a.top_k}, ints.dtype(at::kFloat));
-  Tensor to = at::empty({a.tokens, a.top_k}, ints);
-  Tensor offsets = at::empty({a.experts + 1}, ints);
+  Tensor idx = fresh({a.tokens, a.top_k}, at::kInt, logits);
+  Tensor weights = fresh({a.tokens, a.top_k}, at::kFloat, logits);
+  Tensor to = fresh({a.tokens, a.top_k}, at::kInt, logits);
+  Tensor offsets = fresh({a.experts + 1}, at::kInt, logits);
   const size_t bytes = block::route_workspace(a.tokens, a.experts, a.top_k);
   Tensor workspace;
   if (bytes) {
-    workspace = at::empty({static_cast<int64_t>(bytes)}, ints.dtype(at::kByte));
+    workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, logits);
     a.workspace = workspace.mutable_data_ptr();
   }
   a.idx = idx.mutable_data_ptr<int32_t>();
@@ -171,7 +176,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
     {
       at::NoGradGuard no_grad;
       const Tensor dw = grads[1].contiguous();
-      result[0] = at::empty(saved[0].sizes(), saved[0].options().requires_grad(false), at::MemoryFormat::Contiguous);
+      result[0] = fresh(saved[0].sizes(), saved[0].scalar_type(), saved[0]);
       block::route_topk_backward(a, dw.const_data_ptr<float>(), result[0].mutable_data_ptr(), stream_of(saved[0]));
     }
     once(result);
@@ -236,7 +241,7 @@ void check_move(const char* op, const Tensor& x, const Tensor& rows, const Tenso
 Tensor dispatch_run(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Rows src = as_rows(x);
-  Tensor out = at::empty({rows.numel(), x.size(1)}, x.options().requires_grad(false));
+  Tensor out = fresh({rows.numel(), x.size(1)}, x.scalar_type(), x);
   block::dispatch_rows(move_args(x, rows, offsets), src.ptr(), src.ld, out.mutable_data_ptr(), stream_of(x));
   return out;
 }
@@ -246,7 +251,7 @@ Tensor combine_run(const Tensor& y, const Tensor& weights, const Tensor& rows, c
   const Rows src = as_rows(y);
   block::MoveArgs a = move_args(y, rows, offsets);
   if (weights.defined()) a.weights = weights.const_data_ptr<float>();
-  Tensor out = at::empty({rows.size(0), y.size(1)}, y.options().requires_grad(false));
+  Tensor out = fresh({rows.size(0), y.size(1)}, y.scalar_type(), y);
   block::combine_rows(a, src.ptr(), src.ld, out.mutable_data_ptr(), stream_of(y));
   return out;
 }
@@ -288,8 +293,8 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
       const Rows src = as_rows(y), d = as_rows(grads[0]);
       block::MoveArgs a = move_args(y, rows, offsets);
       a.weights = weights.const_data_ptr<float>();
-      if (ctx->needs_input_grad(0)) result[0] = at::empty(y.sizes(), y.options().requires_grad(false), at::MemoryFormat::Contiguous);
-      if (ctx->needs_input_grad(1)) result[1] = at::empty(weights.sizes(), weights.options().requires_grad(false));
+      if (ctx->needs_input_grad(0)) result[0] = fresh(y.sizes(), y.scalar_type(), y);
+      if (ctx->needs_input_grad(1)) result[1] = fresh(weights.sizes(), at::kFloat, y);
       block::combine_rows_backward(a, src.ptr(), src.ld, d.ptr(), d.ld,
                                    result[0].defined() ? result[0].mutable_data_ptr() : nullptr,
                                    result[1].defined() ? result[1].mutable_data_ptr<float>() : nullptr, stream_of(y));
@@ -369,13 +374,10 @@ NormResult norm_run(const NormCall& c, const Tensor& residual, const Tensor& x, 
   const c10::cuda::CUDAGuard guard(residual.device());
   const NormInputs in(c, residual, x, gamma, post, gate);
   NormResult r;
-  const auto options = residual.options().requires_grad(false);
-  if (x.defined()) r.h = at::empty(residual.sizes(), options, at::MemoryFormat::Contiguous);
-  if (gamma.defined())
-    r.y = at::empty(residual.sizes(), options.dtype(x.defined() ? x.scalar_type() : residual.scalar_type()),
-                    at::MemoryFormat::Contiguous);
-  if (training && post.defined()) r.r1 = at::empty({in.a.rows}, options.dtype(at::kFloat));
-  if (training && gamma.defined()) r.r2 = at::empty({in.a.rows}, options.dtype(at::kFloat));
+  if (x.defined()) r.h = fresh(residual.sizes(), residual.scalar_type(), residual);
+  if (gamma.defined()) r.y = fresh(residual.sizes(), x.defined() ? x.scalar_type() : residual.scalar_type(), residual);
+  if (training && post.defined()) r.r1 = fresh({in.a.rows}, at::kFloat, residual);
+  if (training && gamma.defined()) r.r2 = fresh({in.a.rows}, at::kFloat, residual);
   block::norm_forward(in.a, r.h.defined() ? r.h.mutable_data_ptr() : nullptr,
                       r.y.defined() ? r.y.mutable_data_ptr() : nullptr,
                       r.r1.defined() ? r.r1.mutable_data_ptr<float>() : nullptr,
@@ -434,7 +436,6 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
       if (saved[5].defined()) g.h = saved[5].const_data_ptr();
       if (saved[6].defined()) g.r1 = saved[6].const_data_ptr<float>();
       if (saved[7].defined()) g.r2 = saved[7].const_data_ptr<float>();
-      const auto options = given.options().requires_grad(false);
       size_t edge = 0;
       const bool want_res = ctx->needs_input_grad(edge++);
       const bool want_x = has_x && ctx->needs_input_grad(edge++);
@@ -443,25 +444,25 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
       const bool want_gate = gate.defined() && ctx->needs_input_grad(edge++);
       // Without a gate, a norm behind or a scale both gradients are the same numbers: one is written.
       const bool same = want_res && want_x && !full && xt == rt && in.a.scale == 1.f;
-      const auto fresh = [&](at::ScalarType t) { return at::empty(given.sizes(), options.dtype(t), at::MemoryFormat::Contiguous); };
       if (want_res) {
-        result[0] = fresh(rt);
+        result[0] = fresh(given.sizes(), rt, given);
         g.dresidual = result[0].mutable_data_ptr();
       }
       if (want_x) {
-        result[1] = same ? result[0] : fresh(xt);
+        result[1] = same ? result[0] : fresh(given.sizes(), xt, given);
         if (!same) g.dx = result[1].mutable_data_ptr();
       }
       const bool none = in.a.rows == 0;
-      const auto weight = [&](const Tensor& w) { return none ? at::zeros(w.sizes(), w.options().requires_grad(false))
-                                                             : at::empty(w.sizes(), w.options().requires_grad(false), at::MemoryFormat::Contiguous); };
+      const auto weight = [&](const Tensor& w) {
+        return none ? at::zeros(w.sizes(), w.options().requires_grad(false)) : fresh(w.sizes(), w.scalar_type(), w);
+      };
       if (want_gamma) { result[2] = weight(gamma); g.dgamma = result[2].mutable_data_ptr(); }
       if (want_post) { result[3] = weight(post); g.dpost_gamma = result[3].mutable_data_ptr(); }
       if (want_gate) { result[4] = weight(gate); g.dgate = result[4].mutable_data_ptr(); }
       Tensor workspace;
       if (!none) {
         if (const size_t bytes = block::norm_workspace(in.a, g)) {
-          workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
+          workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, given);
           g.workspace = workspace.mutable_data_ptr();
         }
         block::norm_backward(in.a, g, stream_of(given));

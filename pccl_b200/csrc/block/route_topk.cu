@@ -83,9 +83,18 @@ __device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINIT
 
 __device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
 // For the choice alone.
-__device__ __forceinline__ float quick_sigmoid(float l) { return __fdividef(1.f, 1.f + __expf(-l)); }
+__device__ __forceinline__ float quick_exp(float l) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(l * 1.44269504f));
+  return r;
+}
+__device__ __forceinline__ float quick_sigmoid(float l) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + quick_exp(-l)));
+  return r;
+}
 
-// Bound of the difference of two scores' errors; __expf(x) is off by (2 + 1.2 |x|) 2^-23 of itself.  Sigmoid:
+// Bound of the difference of two scores' errors; quick_exp(x) is off by (2 + 1.2 |x|) 2^-23 of itself.  Sigmoid:
 // p (1 - p) times that is at most 0.7 * 2^-23, the sum and quotient add 2^-22.  Softmax: of the row's largest
 // probability, exponential 5 * 2^-24 (|x| e^-|x| < 0.37), the sum over a lane and the warp (n + 5) 2^-24 and its terms'
 // 5 * 2^-24, quotient and product 3 * 2^-24.
@@ -94,20 +103,9 @@ __device__ __forceinline__ float score_error(bool sigmoid_scores, int n, float l
 }
 
 // ---- a warp per token ------------------------------------------------------------------------------------------
-// Largest first, among equals the lowest number first (comparators keep equals in place only between neighbours, so
-// numbers take part in the comparison where keys are equal).
-template <typename Key, int NE>
-__device__ __forceinline__ void sort_lane(Key (&key)[NE], uint32_t (&num)[NE]) {
-  const auto order = [&](int i, int j) {
-    const bool swap = key[j] > key[i] || (key[j] == key[i] && num[j] < num[i]);
-    const Key k = swap ? key[j] : key[i];
-    const uint32_t n = swap ? num[j] : num[i];
-    key[j] = swap ? key[i] : key[j];
-    num[j] = swap ? num[i] : num[j];
-    key[i] = k;
-    num[i] = n;
-  };
-  // Batcher's odd-even merge sort.
+// Largest first: Batcher's odd-even merge sort.
+template <int NE>
+__device__ __forceinline__ void sort_lane(uint32_t (&key)[NE]) {
 #pragma unroll
   for (int p = 1; p < NE; p *= 2)
 #pragma unroll
@@ -116,7 +114,88 @@ __device__ __forceinline__ void sort_lane(Key (&key)[NE], uint32_t (&num)[NE]) {
       for (int j = k % p; j + k < NE; j += 2 * k)
 #pragma unroll
         for (int i = 0; i < k; ++i)
-          if (i + j + k < NE && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(i + j, i + j + k);
+          if (i + j + k < NE && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t hi = larger(key[i + j], key[i + j + k]);
+            key[i + j + k] = smaller(key[i + j], key[i + j + k]);
+            key[i + j] = hi;
+          }
+}
+
+// Rank of this lane's group score among all, ties to the lower number; group g's score stands in lane g * lanes.
+template <typename Key>
+__device__ __forceinline__ int group_rank(int groups, int lanes, int group, Key mine) {
+  // The lanes of a group share the comparisons.
+  const int lane = threadIdx.x & 31;
+  int rank = 0;
+  for (int g0 = 0; g0 < groups; g0 += lanes) {
+    const int g = g0 + (lane & (lanes - 1));
+    const Key other = __shfl_sync(kAll, mine, g < groups ? g * lanes : 0);
+    rank += g < groups && (other > mine || (other == mine && g < group)) ? 1 : 0;
+  }
+  for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
+  return rank;
+}
+
+// The choice in 32 bits with up to eight experts a lane.  The lowest three bits of a key give way to the expert's
+// place in the lane (lower places larger), so a lane's keys sort with two instructions a comparator and the number
+// comes with the key; lanes compare with those bits set.  That moves a score by less than 2^-20 of itself.  For
+// scores of 16 bits that no bias or sum has touched the bits carry nothing, and the choice is exact (kExact).
+// Results as for choose().
+template <int NE>
+__device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&s)[NE], float tau, bool exact, const float (&l)[NE],
+                                            uint16_t* picked) {
+  const RouteArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  uint32_t key[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) key[j] = (key_of(s[j]) | 7u) ^ static_cast<uint32_t>(j);
+  sort_lane<NE>(key);
+  int close = 0;
+  if (a.top_groups < a.groups) {                   // p.lanes neighbouring lanes a group
+    uint32_t b1 = key[0] | 7u, b2 = NE > 1 ? key[NE > 1 ? 1 : 0] | 7u : 0u;
+    for (int o = 1; o < p.lanes; o <<= 1) {
+      const uint32_t o1 = __shfl_xor_sync(kAll, b1, o), o2 = __shfl_xor_sync(kAll, b2, o);
+      b2 = larger(smaller(b1, o1), larger(b2, o2));
+      b1 = larger(b1, o1);
+    }
+    const int group = lane / p.lanes;
+    const uint32_t mine = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+    const bool real = group < a.groups;
+    const int rank = group_rank(a.groups, p.lanes, group, mine);     // by the whole warp
+    const bool kept = real && rank < a.top_groups;
+    if (!exact) {
+      const float low = value_of(~warp_max(kept ? ~mine : 0u)), high = value_of(warp_max(real && !kept ? mine : 0u));
+      if (!(low - high > 2.f * tau + 0x1p-18f * fabsf(low))) close = 2;
+    }
+    if (a.top2 && a.bias == nullptr) {             // the groups by their sums, the experts by their logits
+#pragma unroll
+      for (int j = 0; j < NE; ++j) key[j] = (key_of(l[j]) | 7u) ^ static_cast<uint32_t>(j);
+      sort_lane<NE>(key);
+    }
+#pragma unroll
+    for (int j = 0; j < NE; ++j) key[j] = kept ? key[j] : 0u;
+  }
+  uint32_t best = key[0] | 7u, won = 0;
+  const int rounds = a.top_k + (exact ? 0 : 1);
+  for (int i = 0; i < rounds; ++i) {
+    const uint32_t m = warp_max(best);
+    won = lane == i ? m : won;
+    const bool own = lane == __ffs(__ballot_sync(kAll, best == m)) - 1;
+    if (own) picked[i] = static_cast<uint16_t>(lane * NE + (~key[0] & 7u));
+#pragma unroll
+    for (int j = 0; j + 1 < NE; ++j) key[j] = own ? key[j + 1] : key[j];
+    key[NE - 1] = own ? 0u : key[NE - 1];
+    best = key[0] | 7u;
+  }
+  __syncwarp();
+  if (!exact) {
+    const uint32_t below = __shfl_down_sync(kAll, won, 1);
+    if (lane < a.top_k && below > 7u) {            // else there is no runner-up
+      const float score = value_of(won);
+      if (!(score - value_of(below) > tau + 0x1p-19f * fabsf(score) + 0x1p-140f)) close |= 1;
+    }
+  }
+  return close;
 }
 
 // Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Expert
@@ -127,16 +206,11 @@ template <typename F, int NE>
 __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], float tau, bool check, const float (&l)[NE],
                                        uint16_t* picked) {
   using Key = decltype(key_of(F()));
-  constexpr bool kSorted = NE <= 8;               // sorting 16 or 32 keys costs more than a few rounds of search
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   Key key[NE];
-  uint32_t num[NE];
 #pragma unroll
-  for (int j = 0; j < NE; ++j) {
-    key[j] = lane * NE + j < a.experts ? key_of(s[j]) : Key(0);
-    num[j] = j;
-  }
+  for (int j = 0; j < NE; ++j) key[j] = key_of(s[j]);
   int close = 0;
   const bool grouped = a.top_groups < a.groups;
   const bool by_logit = a.bias == nullptr && a.top2 && grouped;   // s is not the logits here
@@ -180,11 +254,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
         if (lane == g) mine = score;
       }
     }
-    int rank = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const Key other = __shfl_sync(kAll, mine, p.lanes ? g * p.lanes : g);
-      rank += other > mine || (other == mine && g < group) ? 1 : 0;
-    }
+    const int rank = group_rank(a.groups, p.lanes ? p.lanes : 1, group, mine);
     const bool kept = group < a.groups && rank < a.top_groups;
     if (check) {
       const F low = value_of(static_cast<Key>(~warp_max(kept ? static_cast<Key>(~mine) : Key(0))));
@@ -209,11 +279,6 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
   }
   check = check && a.bias != nullptr;
 
-  if (kSorted) sort_lane<Key, NE>(key, num);
-  uint32_t numbers = 0;                            // four bits each, the head's lowest
-  if (kSorted)
-#pragma unroll
-    for (int j = 0; j < NE; ++j) numbers |= num[j] << (4 * j);
   Key best = 0;
 #pragma unroll
   for (int j = 0; j < NE; ++j) best = larger(best, key[j]);
@@ -223,25 +288,16 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
     const Key m = warp_max(best);
     if (lane == i) won = m;
     if (lane == __ffs(__ballot_sync(kAll, best == m)) - 1) {
-      if constexpr (kSorted) {
-        picked[i] = static_cast<uint16_t>(lane * NE + (numbers & 15u));
-        numbers >>= 4;
+      int at = 0;
 #pragma unroll
-        for (int j = 0; j + 1 < NE; ++j) key[j] = key[j + 1];
-        key[NE - 1] = 0;
-        best = key[0];
-      } else {
-        int at = 0;
+      for (int j = NE - 1; j >= 0; --j)
+        if (key[j] == m) at = j;
+      picked[i] = static_cast<uint16_t>(lane * NE + at);
+      best = 0;
 #pragma unroll
-        for (int j = NE - 1; j >= 0; --j)
-          if (key[j] == m) at = j;
-        picked[i] = static_cast<uint16_t>(lane * NE + at);
-        best = 0;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          if (j == at) key[j] = 0;
-          best = larger(best, key[j]);
-        }
+      for (int j = 0; j < NE; ++j) {
+        if (j == at) key[j] = 0;
+        best = larger(best, key[j]);
       }
     }
   }
@@ -256,15 +312,28 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
   return close;
 }
 
+// choose() out of line: groups that do not fall into whole lanes are rare, and should not cost the others registers.
+template <int NE>
+__device__ __noinline__ int choose_ragged(const RouteParams& p, const float (&s)[NE], float tau, bool check, const float (&l)[NE],
+                                          uint16_t* picked) {
+  return choose<float, NE>(p, s, tau, check, l, picked);
+}
+
 // The same choice from scores in 64 bits.
 template <int NE>
 __device__ __noinline__ void choose_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
   const RouteArgs& a = p.a;
+  double s[NE], total = 0;
+  if (a.bias == nullptr && !(a.top2 && a.top_groups < a.groups)) {
+#pragma unroll
+    for (int j = 0; j < NE; ++j) s[j] = static_cast<double>(l[j]);
+    choose<double, NE>(p, s, 0.f, false, l, picked);
+    return;
+  }
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < NE; ++j) top = fmaxf(top, l[j]);
   top = warp_max(top);
-  double s[NE], total = 0;
 #pragma unroll
   for (int j = 0; j < NE; ++j) {
     const double v = static_cast<double>(l[j]);
@@ -286,10 +355,10 @@ __device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int 
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   float l = 0.f, b = 0.f;
-  if (a.bias != nullptr && lane <= a.top_k && lane < a.experts) {
+  if (lane <= a.top_k && lane < a.experts) {
     const int e = min(static_cast<int>(picked[lane]), a.experts - 1);
     l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
-    b = a.bias[e];
+    b = a.bias != nullptr ? a.bias[e] : 0.f;
   }
   const float l1 = __shfl_down_sync(kAll, l, 1), b1 = __shfl_down_sync(kAll, b, 1);
   return !__any_sync(kAll, (close & 2) || ((close & 1) && !(l == l1 && b == b1)));
@@ -298,6 +367,15 @@ __device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int 
 // A lane's share of a row as it lies in memory.
 template <typename T, int NE> struct alignas(NE * sizeof(T) > 16 ? 16 : NE * sizeof(T)) Share { T v[NE]; };
 
+// Lanes and places beyond the last expert hold minus infinity: they have the highest numbers, so among equals every
+// expert comes before them, and there are always enough experts.
+template <typename T> __device__ __forceinline__ T lowest_value() { return from_f32<T>(-INFINITY); }
+template <typename T, int NE> __device__ __forceinline__ Share<T, NE> empty_share() {
+  Share<T, NE> r;
+#pragma unroll
+  for (int j = 0; j < NE; ++j) r.v[j] = lowest_value<T>();
+  return r;
+}
 template <typename T, int NE>
 __device__ __forceinline__ void load_share(const RouteParams& p, int64_t t, Share<T, NE>* to) {
   const RouteArgs& a = p.a;
@@ -307,15 +385,14 @@ __device__ __forceinline__ void load_share(const RouteParams& p, int64_t t, Shar
     if (e0 < a.experts) *to = *reinterpret_cast<const Share<T, NE>*>(row + e0);
   } else {
 #pragma unroll
-    for (int j = 0; j < NE; ++j) to->v[j] = row[min(e0 + j, a.experts - 1)];
+    for (int j = 0; j < NE; ++j)
+      if (e0 + j < a.experts) to->v[j] = row[e0 + j];
   }
 }
-// Cleaned logits, -infinity beyond the last expert.
 template <typename T, int NE>
-__device__ __forceinline__ void clean_share(const RouteArgs& a, const Share<T, NE>& from, float (&l)[NE]) {
-  const int e0 = (threadIdx.x & 31) * NE;
+__device__ __forceinline__ void clean_share(const Share<T, NE>& from, float (&l)[NE]) {
 #pragma unroll
-  for (int j = 0; j < NE; ++j) l[j] = e0 + j < a.experts ? clean(to_f32<T>(from.v[j])) : -INFINITY;
+  for (int j = 0; j < NE; ++j) l[j] = clean(to_f32<T>(from.v[j]));
 }
 
 // Shares of the choices among themselves, sum 1 (0 where every chosen logit is -infinity).  Scaled by the
@@ -324,7 +401,9 @@ __device__ __forceinline__ void clean_share(const RouteArgs& a, const Share<T, N
 __device__ __forceinline__ float share_size(bool sigmoid_scores, float l, float top) {
   if (l == -INFINITY) return 0.f;
   if (!sigmoid_scores) return expf(l - top);
-  return l > 0.f ? sigmoid(l) : expf(l - fminf(top, 0.f)) / (1.f + expf(l));
+  const float e = expf(-fabsf(l));
+  const float up = l > 0.f ? 1.f : top > 0.f ? e : expf(l - top);
+  return up / (1.f + e);
 }
 __device__ __forceinline__ float share(const RouteArgs& a, float l) {
   if (static_cast<int>(threadIdx.x & 31) >= a.top_k) l = -INFINITY;
@@ -415,7 +494,7 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
   uint16_t* const picked = picks[warp];
   asm volatile("griddepcontrol.launch_dependents;");
 
-  Share<T, NE> next{};
+  Share<T, NE> next = empty_share<T, NE>();
   if (warp < count) load_share<T, NE>(p, first + warp, &next);
   float bias[NE];
 #pragma unroll
@@ -433,10 +512,8 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
     float w = 0.f;
     if (a.mask == nullptr || a.mask[t]) {
       float l[NE], s[NE];
-      clean_share<T, NE>(a, raw, l);
-      float top = 0.f, total = 1.f;
-#pragma unroll
-      for (int j = 0; j < NE; ++j) s[j] = l[j];
+      clean_share<T, NE>(raw, l);
+      float top = 0.f, total = 1.f, tau = 0.f;
       if (!a.sigmoid && (scored || !a.renormalise)) {
         top = l[0];
 #pragma unroll
@@ -446,7 +523,7 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
 #pragma unroll
         for (int j = 0; j < NE; ++j) {
           // The weights are made of these where they are not renormalised: then to the full 2^-22.
-          const float x = a.renormalise ? __expf(l[j] - top) : expf(l[j] - top);
+          const float x = a.renormalise ? quick_exp(l[j] - top) : expf(l[j] - top);
           s[j] = l[j] == -INFINITY ? 0.f : x;
           total += s[j];
         }
@@ -459,11 +536,19 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
           const float prob = a.sigmoid ? quick_sigmoid(l[j]) : s[j] * inv;
           s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
         }
-        const int close = choose<float, NE>(p, s, score_error(a.sigmoid, NE, inv), true, l, picked);
-        if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, picked)) choose_wide<NE>(p, l, bias, picked);
+        tau = score_error(a.sigmoid, NE, inv);
       } else {
-        choose<float, NE>(p, l, 0.f, false, l, picked);
+#pragma unroll
+        for (int j = 0; j < NE; ++j) s[j] = l[j];
       }
+      int close;
+      if constexpr (NE <= 8) {
+        if (a.top_groups == a.groups || p.lanes) close = choose_quick<NE>(p, s, tau, sizeof(T) == 2 && !scored, l, picked);
+        else close = choose_ragged<NE>(p, s, tau, scored, l, picked);
+      } else {
+        close = choose<float, NE>(p, s, tau, scored, l, picked);
+      }
+      if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, picked)) choose_wide<NE>(p, l, bias, picked);
       e = lane < a.top_k ? picked[lane] : -1;
       const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
       if (a.renormalise) w = share(a, le);
@@ -473,8 +558,9 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
       __syncwarp();                                                  // picked is read
     }
     if (lane < a.top_k) {
-      a.idx[t * a.top_k + lane] = e;
-      a.weights[t * a.top_k + lane] = w;
+      const int at = (first + i) * a.top_k + lane;
+      a.idx[at] = e;
+      a.weights[at] = w;
       chosen[i * a.top_k + lane] = static_cast<uint16_t>(e);           // 0xffff: none
       if (e >= 0) atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
     }
@@ -767,10 +853,10 @@ __global__ void __launch_bounds__(256) route_warp_backward_kernel(const RoutePar
       if (e >= 0 && le != -INFINITY) row[e] = from_f32<T>(d);
       continue;
     }
-    Share<T, NE> raw;
+    Share<T, NE> raw = empty_share<T, NE>();
     load_share<T, NE>(p, t, &raw);
     float l[NE];
-    clean_share<T, NE>(a, raw, l);
+    clean_share<T, NE>(raw, l);
     float top = l[0], total = 0.f;
 #pragma unroll
     for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
