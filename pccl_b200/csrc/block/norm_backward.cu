@@ -24,14 +24,14 @@ template <typename TX, typename TR, bool kFull> struct BackwardSlots {
   static constexpr int kGamma = 0, kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
   static constexpr int kDy = kBytes<TR>, kH = kDy + kBytes<TX>, kX = kH + kBytes<TR>;
   static constexpr int kShare = kX + (kReadsX ? kBytes<TX> : 0);
-  static int window(int n) { return 2 * window_bytes<TR>(n) + (kReadsX ? 2 : 1) * window_bytes<TX>(n); }
+  static int window(int threads) { return 2 * window_bytes<TR>(threads) + (kReadsX ? 2 : 1) * window_bytes<TX>(threads); }
 };
 
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void store_weight_grad(void* out, int f32, int64_t first, int n, int tid, int width,
+__device__ __forceinline__ void store_weight_grad(void* out, int f32, int64_t first, const Columns<kVec, G>& c,
                                                   const float2* f) {
-  if (f32) store_row<float, kVec, G>(static_cast<float*>(out) + first, n, tid, width, f);
-  else store_row<T, kVec, G>(static_cast<T*>(out) + first, n, tid, width, f);
+  if (f32) store_row<float, kVec, G>(static_cast<float*>(out) + first, c, f);
+  else store_row<T, kVec, G>(static_cast<T*>(out) + first, c, f);
 }
 
 template <typename TX, typename TR, int kMode, bool kFull, int kMost>
@@ -45,13 +45,14 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
   const NormGrads& g = p.g;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
+  const Columns<kVec, G> c(n);
   row_sum_clear(sums);
   const int64_t begin = run_start(a.rows, p.workers, blockIdx.x), end = run_start(a.rows, p.workers, blockIdx.x + 1);
 
   char* const gammas = smem;
   char* const g1 = smem + Slots::kG1 * width;
   char* const ring = smem + Slots::kWeights * width;
-  const int wx = window_bytes<TX>(n), wr = window_bytes<TR>(n);
+  const int wx = window_bytes<TX>(width), wr = window_bytes<TR>(width);
   const int stage = kMode == kRing ? Slots::kShare * width : 2 * wr + (Slots::kReadsX ? 2 : 1) * wx;
   const int off_dy = kMode == kRing ? Slots::kDy * width : wr;
   const int off_h = kMode == kRing ? Slots::kH * width : wr + wx;
@@ -67,19 +68,19 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
     if (row < end) {
       char* to = ring + s * stage;
       if constexpr (kMode == kRing) {
-        if (g.dh) fetch_share<TR, G>(to, dh_rows + row * g.lddh, n, tid, width);
+        if (g.dh) fetch_share<TR, G>(to, dh_rows + row * g.lddh, c);
         if (g.dy) {
-          fetch_share<TX, G>(to + off_dy, dy_rows + row * g.lddy, n, tid, width);
-          fetch_share<TR, G>(to + off_h, stream + row * lds, n, tid, width);
+          fetch_share<TX, G>(to + off_dy, dy_rows + row * g.lddy, c);
+          fetch_share<TR, G>(to + off_h, stream + row * lds, c);
         }
-        if (reads_x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, n, tid, width);
+        if (reads_x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, c);
       } else {
-        if (g.dh) fetch_window(to, dh_rows + row * g.lddh, n, tid, width);
+        if (g.dh) fetch_window(to, dh_rows + row * g.lddh, n);
         if (g.dy) {
-          fetch_window(to + off_dy, dy_rows + row * g.lddy, n, tid, width);
-          fetch_window(to + off_h, stream + row * lds, n, tid, width);
+          fetch_window(to + off_dy, dy_rows + row * g.lddy, n);
+          fetch_window(to + off_h, stream + row * lds, n);
         }
-        if (reads_x) fetch_window(to + off_x, x_rows + row * a.ldx, n, tid, width);
+        if (reads_x) fetch_window(to + off_x, x_rows + row * a.ldx, n);
       }
     }
     copies_commit();
@@ -95,15 +96,15 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
   }
   if (a.gamma.ptr) {
     float2 w[kHeld / 2];
-    load_weight<TX, kVec, G>(a.gamma, 0, n, tid, width, w);
-    slots_store(gammas, tid, width, w);
+    load_weight<TX, kVec, G>(a.gamma, 0, c, w);
+    slots_store(gammas, w);
   }
   bool first = true;                               // no group has ended yet
   int64_t group = 0, left = 0;                     // rows left of the present group of rows that share a gate
   if constexpr (kFull) {
     group = a.gate.ptr ? begin / a.gate_rows : 0;
     left = a.gate.ptr ? (group + 1) * a.gate_rows - begin : a.rows;
-    form_g1<TX, kVec, G>(a, group, g1, tid, width);
+    form_g1<TX, kVec, G>(a, group, g1, c);
   }
   float next_r1 = kFull && a.post_gamma.ptr ? g.r1[begin] : 1.f;
   float next_r2 = g.dy ? g.r2[begin] : 0.f;
@@ -136,19 +137,19 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
       for (int v = 0; v < kGroups; ++v) {
         float2 f[G / 2], w[G / 2];
         float2* const h = n2 + v * (G / 2);
-        take<TR, kMode, G>(held + off_h, stream + t * lds, v, n, tid, width, h);
+        take<TR, kMode, G>(held + off_h, stream + t * lds, v, c, h);
         if (Slots::kReadsX && reads_x && !g.h) {
-          take<TX, kMode, G>(held + off_x, row_x, v, n, tid, width, f);
+          take<TX, kMode, G>(held + off_x, row_x, v, c, f);
           if (kFull) {
-            slots_load<G>(g1, v, tid, width, w);
+            slots_load<G>(g1, v, w);
 #pragma unroll
             for (int j = 0; j < G / 2; ++j) f[j] = mul2(mul2(f[j], both(r1)), w[j]);
           }
 #pragma unroll
           for (int j = 0; j < G / 2; ++j) h[j] = fma2(both(a.scale), h[j], f[j]);
         }
-        take<TX, kMode, G>(held + off_dy, dy_rows + t * g.lddy, v, n, tid, width, f);
-        slots_load<G>(gammas, v, tid, width, w);
+        take<TX, kMode, G>(held + off_dy, dy_rows + t * g.lddy, v, c, f);
+        slots_load<G>(gammas, v, w);
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) {
           h[j] = mul2(h[j], both(r2));
@@ -169,18 +170,18 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
     for (int v = 0; v < kGroups; ++v) {
       float2 f[G / 2], w[G / 2];
       if (g.dh) {
-        take<TR, kMode, G>(held, dh_rows + t * g.lddh, v, n, tid, width, f);
+        take<TR, kMode, G>(held, dh_rows + t * g.lddh, v, c, f);
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) d[v * (G / 2) + j] = add2(d[v * (G / 2) + j], f[j]);
       }
       if (g.dresidual) {
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) f[j] = mul2(both(a.scale), d[v * (G / 2) + j]);
-        store_group<TR, kVec, G>(static_cast<TR*>(g.dresidual) + t * n, v, n, tid, width, f);
+        store_group<TR, kVec, G>(static_cast<TR*>(g.dresidual) + t * n, v, c, f);
       }
       if constexpr (kFull) {
-        take<TX, kMode, G>(held + off_x, row_x, v, n, tid, width, f);
-        slots_load<G>(g1, v, tid, width, w);
+        take<TX, kMode, G>(held + off_x, row_x, v, c, f);
+        slots_load<G>(g1, v, w);
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) {
           f[j] = mul2(f[j], both(r1));
@@ -197,15 +198,15 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
 #pragma unroll
         for (int v = 0; v < kGroups; ++v) {
           float2 f[G / 2];
-          take<TX, kMode, G>(held + off_x, row_x, v, n, tid, width, f);
+          take<TX, kMode, G>(held + off_x, row_x, v, c, f);
 #pragma unroll
           for (int j = 0; j < G / 2; ++j) f[j] = fma2(both(r1), d[v * (G / 2) + j], mul2(both(pull), f[j]));
-          store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, f);
+          store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, c, f);
         }
       }
     } else if (g.dx) {
 #pragma unroll
-      for (int v = 0; v < kGroups; ++v) store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, n, tid, width, d + v * (G / 2));
+      for (int v = 0; v < kGroups; ++v) store_group<TX, kVec, G>(static_cast<TX*>(g.dx) + t * n, v, c, d + v * (G / 2));
     }
     if constexpr (kFull) {
       if (--left == 0 || t + 1 == end) {
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
             if (p.part_post) {
               // Added up in this thread's own columns of the block's part: once a group, so not worth registers.
               float* const part = p.part_post + static_cast<int64_t>(blockIdx.x) * n;
-              load_weight<TX, kVec, G>(a.gate, group * n, n, tid, width, w);
+              load_weight<TX, kVec, G>(a.gate, group * n, c, w);
 #pragma unroll
               for (int v = 0; v < kGroups; ++v) {
                 float2 sum[G / 2];
@@ -224,39 +225,39 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
 #pragma unroll
                   for (int j = 0; j < G / 2; ++j) sum[j] = both(0.f);
                 } else {
-                  load_group<float, kVec, G>(part, v, n, tid, width, sum);
+                  load_group<float, kVec, G>(part, v, c, sum);
                 }
 #pragma unroll
                 for (int j = 0; j < G / 2; ++j) sum[j] = fma2(w[v * (G / 2) + j], acc_s[v * (G / 2) + j], sum[j]);
-                store_group<float, kVec, G>(part, v, n, tid, width, sum);
+                store_group<float, kVec, G>(part, v, c, sum);
               }
               first = false;
             }
-            load_weight<TX, kVec, G>(a.post_gamma, 0, n, tid, width, w);
+            load_weight<TX, kVec, G>(a.post_gamma, 0, c, w);
 #pragma unroll
             for (int i = 0; i < kHeld / 2; ++i) acc_s[i] = mul2(acc_s[i], w[i]);
           }
           if (g.dgate) {
             if (group * a.gate_rows >= begin && (group + 1) * a.gate_rows <= end) {
-              store_weight_grad<TX, kVec, G>(g.dgate, a.gate.f32, group * n, n, tid, width, acc_s);
+              store_weight_grad<TX, kVec, G>(g.dgate, a.gate.f32, group * n, c, acc_s);
             } else {
               const int slot = group * a.gate_rows <= begin ? 0 : 1;
-              store_row<float, kVec, G>(p.part_gate + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * n, n, tid, width, acc_s);
+              store_row<float, kVec, G>(p.part_gate + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * n, c, acc_s);
             }
           }
 #pragma unroll
           for (int i = 0; i < kHeld / 2; ++i) acc_s[i] = both(0.f);
-          if (t + 1 < end) form_g1<TX, kVec, G>(a, ++group, g1, tid, width);
+          if (t + 1 < end) form_g1<TX, kVec, G>(a, ++group, g1, c);
           left = a.gate_rows;
         }
       }
     }
   }
   if constexpr (kMode == kRing || kMode == kWindow) copies_wait(0);
-  if (p.part_gamma) store_row<float, kVec, G>(p.part_gamma + static_cast<int64_t>(blockIdx.x) * n, n, tid, width, acc_gamma);
+  if (p.part_gamma) store_row<float, kVec, G>(p.part_gamma + static_cast<int64_t>(blockIdx.x) * n, c, acc_gamma);
   if constexpr (kFull) {
     if (p.part_post && !a.gate.ptr) {
-      store_row<float, kVec, G>(p.part_post + static_cast<int64_t>(blockIdx.x) * n, n, tid, width, acc_s);
+      store_row<float, kVec, G>(p.part_post + static_cast<int64_t>(blockIdx.x) * n, c, acc_s);
     }
   }
 }
@@ -324,7 +325,7 @@ int worker_count(const NormArgs& a) {
 template <typename TX, typename TR, bool kFull, int kMost>
 void backward_mode(NormParams& p, bool vec, int threads, cudaStream_t stream) {
   using Slots = BackwardSlots<TX, TR, kFull>;
-  const RingSize size{threads, Slots::kWeights, Slots::kShare, Slots::window(p.a.hidden)};
+  const RingSize size{threads, Slots::kWeights, Slots::kShare, Slots::window(threads)};
   size_t smem = 0;
   switch (choose_mode(size, vec, &p.ring, &smem)) {
     case kRing: launch(norm_backward_kernel<TX, TR, kRing, kFull, kMost>, p, threads, smem, stream); break;

@@ -42,11 +42,17 @@ struct NormParams {
   int ring;                   // rows in shared memory
 };
 
-// Column of value j of group v held by a thread: G in a row where rows are aligned, else a thread's values stand a
-// whole row of threads apart, so that neighbours read neighbours.
-template <bool kVec, int G> __device__ __forceinline__ int column(int v, int j, int tid, int width) {
-  return kVec ? (v * width + tid) * G + j : (v * G + j) * width + tid;
-}
+// A warp holds 32 * kHeld consecutive columns: where rows are aligned a lane has G neighbours of every 32 * G of them,
+// else one of every 32.  Steps from one access to the next are constants then, which matters: with a step of the
+// block's width a third of all instructions were addresses.
+template <bool kVec, int G> struct Columns {
+  int first;                  // this thread's first column
+  int room;                   // columns from there to the row's end
+  __device__ explicit Columns(int hidden) {
+    first = static_cast<int>(threadIdx.x >> 5) * 32 * kHeld + static_cast<int>(threadIdx.x & 31) * (kVec ? G : 1);
+    room = hidden - first;
+  }
+};
 
 // G values as they lie in memory.
 template <typename T, int G> struct alignas(G * sizeof(T) > 16 ? 16 : G * sizeof(T)) Raw { uint32_t w[G * sizeof(T) / 4]; };
@@ -74,11 +80,10 @@ template <typename T, int G> __device__ __forceinline__ Raw<T, G> pack(const flo
 
 // The values of group v, from the row itself.
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void load_group(const T* row, int v, int hidden, int tid, int width, float2* to) {
+__device__ __forceinline__ void load_group(const T* row, int v, const Columns<kVec, G>& c, float2* to) {
   if constexpr (kVec) {
-    const int at = (v * width + tid) * G;
-    if (at < hidden) {
-      unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(row + at), to);
+    if (v * 32 * G < c.room) {
+      unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(row + c.first + v * 32 * G), to);
     } else {
 #pragma unroll
       for (int j = 0; j < G / 2; ++j) to[j] = make_float2(0.f, 0.f);
@@ -86,45 +91,39 @@ __device__ __forceinline__ void load_group(const T* row, int v, int hidden, int 
   } else {
     float* f = reinterpret_cast<float*>(to);
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int at = column<false, G>(v, j, tid, width);
-      f[j] = at < hidden ? to_f32<T>(row[at]) : 0.f;
-    }
+    for (int j = 0; j < G; ++j) f[j] = (v * G + j) * 32 < c.room ? to_f32<T>((row + c.first)[(v * G + j) * 32]) : 0.f;
   }
 }
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void store_group(T* row, int v, int hidden, int tid, int width, const float2* from) {
+__device__ __forceinline__ void store_group(T* row, int v, const Columns<kVec, G>& c, const float2* from) {
   if constexpr (kVec) {
-    const int at = (v * width + tid) * G;
-    if (at < hidden) *reinterpret_cast<Raw<T, G>*>(row + at) = pack<T, G>(from);
+    if (v * 32 * G < c.room) *reinterpret_cast<Raw<T, G>*>(row + c.first + v * 32 * G) = pack<T, G>(from);
   } else {
     const float* f = reinterpret_cast<const float*>(from);
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int at = column<false, G>(v, j, tid, width);
-      if (at < hidden) row[at] = from_f32<T>(f[j]);
-    }
+    for (int j = 0; j < G; ++j)
+      if ((v * G + j) * 32 < c.room) (row + c.first)[(v * G + j) * 32] = from_f32<T>(f[j]);
   }
 }
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void store_row(T* row, int hidden, int tid, int width, const float2* f) {
+__device__ __forceinline__ void store_row(T* row, const Columns<kVec, G>& c, const float2* f) {
 #pragma unroll
-  for (int v = 0; v < kHeld / G; ++v) store_group<T, kVec, G>(row, v, hidden, tid, width, f + v * (G / 2));
+  for (int v = 0; v < kHeld / G; ++v) store_group<T, kVec, G>(row, v, c, f + v * (G / 2));
 }
 // A weight vector is of the activations' type or of 32 bits.
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void load_weight(const Weight& w, int64_t first, int hidden, int tid, int width, float2* f) {
+__device__ __forceinline__ void load_weight(const Weight& w, int64_t first, const Columns<kVec, G>& c, float2* f) {
 #pragma unroll
   for (int v = 0; v < kHeld / G; ++v) {
-    if (w.f32) load_group<float, kVec, G>(static_cast<const float*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
-    else load_group<T, kVec, G>(static_cast<const T*>(w.ptr) + first, v, hidden, tid, width, f + v * (G / 2));
+    if (w.f32) load_group<float, kVec, G>(static_cast<const float*>(w.ptr) + first, v, c, f + v * (G / 2));
+    else load_group<T, kVec, G>(static_cast<const T*>(w.ptr) + first, v, c, f + v * (G / 2));
   }
 }
 
 // ---- ring ------------------------------------------------------------------------------------------------
-// A thread's share of a row of T: kHeld values.  A weight's slots and (mode kRing) a row's stand group by group, the
-// threads' next to one another: a warp's copies then fill whole lines of shared memory.  (With each thread's slots
-// in one piece the copies of neighbours went to different lines, and every kernel here took a quarter longer.)
+// A thread's share of a row of T: kHeld values.  In the ring a row is an image of itself, so a warp's copies fill whole
+// lines of shared memory.  (With each thread's share in one piece the copies of neighbours went to different lines,
+// and every kernel here took a quarter longer.)
 template <typename T> constexpr int kBytes = kHeld * static_cast<int>(sizeof(T));
 
 // The first `size` of kSize bytes (8 or 16), and zeros for the rest.
@@ -145,43 +144,45 @@ __device__ __forceinline__ void copies_wait(int left) {
 }
 
 template <typename T, int G>
-__device__ __forceinline__ void fetch_share(char* slot, const T* row, int hidden, int tid, int width) {
+__device__ __forceinline__ void fetch_share(char* image, const T* row, const Columns<true, G>& c) {
+  constexpr int kSize = G * static_cast<int>(sizeof(T));
 #pragma unroll
   for (int v = 0; v < kHeld / G; ++v) {
-    const int at = (v * width + tid) * G;
-    const bool beyond = at >= hidden;
-    constexpr int kSize = G * static_cast<int>(sizeof(T));
-    copy_async<kSize>(slot + (v * width + tid) * kSize, row + (beyond ? 0 : at), beyond ? 0 : kSize);
+    const bool beyond = v * 32 * G >= c.room;
+    copy_async<kSize>(image + c.first * static_cast<int>(sizeof(T)) + v * 32 * kSize, beyond ? row : row + c.first + v * 32 * G,
+                      beyond ? 0 : kSize);
   }
 }
 
 // Bytes of a window for any row of T.
-template <typename T> __host__ __device__ constexpr int window_bytes(int hidden) {
-  return (hidden * static_cast<int>(sizeof(T)) + 15) / 16 * 16 + 16;
-}
-// The 16-byte blocks that cover the row.  The first may begin with values in front of it: such a block holds a value
-// of the row, and allocations begin at multiples of 256 bytes, so all of it is theirs.  Nothing is read behind.
+template <typename T> __host__ __device__ constexpr int window_bytes(int threads) { return threads * kBytes<T> + 16; }
+// The 16-byte blocks that cover the row, and zeros up to the last column that a thread holds.  The first may begin with
+// values in front of the row: such a block holds a value of the row, and allocations begin at multiples of 256
+// bytes, so all of it is theirs.  Nothing is read behind the row.
 template <typename T>
-__device__ __forceinline__ void fetch_window(char* window, const T* row, int hidden, int tid, int width) {
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(row), end = begin + static_cast<uintptr_t>(hidden) * sizeof(T);
-  const uintptr_t first = begin & ~static_cast<uintptr_t>(15);
-  const int blocks = static_cast<int>((end - first + 15) / 16);
-  for (int i = tid; i < blocks; i += width) {
-    const uintptr_t from = first + static_cast<uintptr_t>(i) * 16;
-    copy_async<16>(window + i * 16, reinterpret_cast<const void*>(from), static_cast<int>(min(end - from, static_cast<uintptr_t>(16))));
+__device__ __forceinline__ void fetch_window(char* window, const T* row, int hidden) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(row);
+  const int ahead = static_cast<int>(begin & 15), bytes = ahead + hidden * static_cast<int>(sizeof(T));
+  const char* const first = reinterpret_cast<const char*>(begin - ahead);
+  const int all = window_bytes<T>(static_cast<int>(blockDim.x));
+  for (int at = static_cast<int>(threadIdx.x) * 16; at < all; at += static_cast<int>(blockDim.x) * 16) {
+    const int size = min(max(bytes - at, 0), 16);
+    copy_async<16>(window + at, size > 0 ? first + at : first, size);
   }
 }
 
-// Group v of a row of T: `slot` is the row's place in the ring, or the window.
+// Group v of a row of T; `held` is the row's image in the ring, or its window.
 template <typename T, int kMode, int G>
-__device__ __forceinline__ void take(const char* slot, const T* row, int v, int hidden, int tid, int width, float2* to) {
+__device__ __forceinline__ void take(const char* held, const T* row, int v, const Columns<aligned_mode(kMode), G>& c, float2* to) {
   if constexpr (kMode == kRing) {
-    unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(slot + (v * width + tid) * static_cast<int>(G * sizeof(T))), to);
+    unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(held + c.first * static_cast<int>(sizeof(T)) + v * static_cast<int>(32 * G * sizeof(T))), to);
   } else if constexpr (kMode == kWindow) {
-    const T* at = reinterpret_cast<const T*>(slot + (reinterpret_cast<uintptr_t>(row) & 15));
-    load_group<T, false, G>(at, v, hidden, tid, width, to);
+    const T* at = reinterpret_cast<const T*>(held + (reinterpret_cast<uintptr_t>(row) & 15)) + c.first;
+    float* f = reinterpret_cast<float*>(to);
+#pragma unroll
+    for (int j = 0; j < G; ++j) f[j] = to_f32<T>(at[(v * G + j) * 32]);
   } else {
-    load_group<T, kMode == kDirect, G>(row, v, hidden, tid, width, to);
+    load_group<T, kMode == kDirect, G>(row, v, c, to);
   }
 }
 
@@ -209,15 +210,17 @@ __device__ __forceinline__ float row_sum(float v, RowSums& sums, int* turn) {
 }
 
 // A weight's slots: kHeld 32-bit values, four to an access.
-__device__ __forceinline__ void slots_store(char* slot, int tid, int width, const float2* f) {
+__device__ __forceinline__ int slot_place() { return static_cast<int>(threadIdx.x >> 5) * 8 * kHeld + static_cast<int>(threadIdx.x & 31); }
+__device__ __forceinline__ void slots_store(char* slots, const float2* f) {
+  float4* const at = reinterpret_cast<float4*>(slots) + slot_place();
 #pragma unroll
-  for (int i = 0; i < kHeld / 4; ++i)
-    reinterpret_cast<float4*>(slot)[i * width + tid] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
+  for (int i = 0; i < kHeld / 4; ++i) at[i * 32] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
 }
-template <int G> __device__ __forceinline__ void slots_load(const char* slot, int v, int tid, int width, float2* f) {
+template <int G> __device__ __forceinline__ void slots_load(const char* slots, int v, float2* f) {
+  const float4* const at = reinterpret_cast<const float4*>(slots) + slot_place();
 #pragma unroll
   for (int i = 0; i < G / 4; ++i) {
-    const float4 q = reinterpret_cast<const float4*>(slot)[(v * (G / 4) + i) * width + tid];
+    const float4 q = at[(v * (G / 4) + i) * 32];
     f[2 * i] = make_float2(q.x, q.y);
     f[2 * i + 1] = make_float2(q.z, q.w);
   }
@@ -225,15 +228,15 @@ template <int G> __device__ __forceinline__ void slots_load(const char* slot, in
 
 // g1 = post_gamma * gate of one group of rows into its slots (what is absent counts as 1).
 template <typename T, bool kVec, int G>
-__device__ __forceinline__ void form_g1(const NormArgs& a, int64_t group, char* slot, int tid, int width) {
+__device__ __forceinline__ void form_g1(const NormArgs& a, int64_t group, char* slots, const Columns<kVec, G>& c) {
   float2 f[kHeld / 2], w[kHeld / 2];
-  if (a.post_gamma.ptr) load_weight<T, kVec, G>(a.post_gamma, 0, a.hidden, tid, width, f);
+  if (a.post_gamma.ptr) load_weight<T, kVec, G>(a.post_gamma, 0, c, f);
   if (a.gate.ptr) {
-    load_weight<T, kVec, G>(a.gate, group * a.hidden, a.hidden, tid, width, w);
+    load_weight<T, kVec, G>(a.gate, group * a.hidden, c, w);
 #pragma unroll
     for (int i = 0; i < kHeld / 2; ++i) f[i] = a.post_gamma.ptr ? mul2(f[i], w[i]) : w[i];
   }
-  slots_store(slot, tid, width, f);
+  slots_store(slots, f);
 }
 
 // First row of worker w's run; w = workers gives the number of rows.

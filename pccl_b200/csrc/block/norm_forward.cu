@@ -29,25 +29,26 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
   const NormArgs& a = p.a;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
+  const Columns<kVec, G> c(n);
   row_sum_clear(sums);
   const int64_t begin = run_start(a.rows, p.workers, blockIdx.x), end = run_start(a.rows, p.workers, blockIdx.x + 1);
 
   char* const gammas = smem;
   char* const g1 = smem + Slots::kG1 * width;
   char* const ring = smem + Slots::kWeights * width;
-  const int stage = kMode == kRing ? Slots::kShare * width : window_bytes<TR>(n) + window_bytes<TX>(n);
-  const int off_x = kMode == kRing ? Slots::kX * width : window_bytes<TR>(n);
+  const int stage = kMode == kRing ? Slots::kShare * width : window_bytes<TR>(width) + window_bytes<TX>(width);
+  const int off_x = kMode == kRing ? Slots::kX * width : window_bytes<TR>(width);
   const TR* const residual = static_cast<const TR*>(a.residual);
   const TX* const x_rows = static_cast<const TX*>(a.x);
   const auto fetch = [&](int64_t row, int s) {
     if (row < end) {
       char* to = ring + s * stage;
       if constexpr (kMode == kRing) {
-        fetch_share<TR, G>(to, residual + row * a.ldr, n, tid, width);
-        if (a.x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, n, tid, width);
+        fetch_share<TR, G>(to, residual + row * a.ldr, c);
+        if (a.x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, c);
       } else {
-        fetch_window(to, residual + row * a.ldr, n, tid, width);
-        if (a.x) fetch_window(to + off_x, x_rows + row * a.ldx, n, tid, width);
+        fetch_window(to, residual + row * a.ldr, n);
+        if (a.x) fetch_window(to + off_x, x_rows + row * a.ldx, n);
       }
     }
     copies_commit();
@@ -57,14 +58,14 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
 
   if (a.gamma.ptr) {
     float2 w[kHeld / 2];
-    load_weight<TX, kVec, G>(a.gamma, 0, n, tid, width, w);
-    slots_store(gammas, tid, width, w);
+    load_weight<TX, kVec, G>(a.gamma, 0, c, w);
+    slots_store(gammas, w);
   }
   int64_t group = 0, left = 0;                     // rows left of the present group of rows that share a gate
   if constexpr (kFull) {
     group = a.gate.ptr ? begin / a.gate_rows : 0;
     left = a.gate.ptr ? (group + 1) * a.gate_rows - begin : a.rows;
-    form_g1<TX, kVec, G>(a, group, g1, tid, width);
+    form_g1<TX, kVec, G>(a, group, g1, c);
   }
 
   int turn = 0, s = 0;
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
       float2 ss = both(0.f);
 #pragma unroll
       for (int v = 0; v < kGroups; ++v) {
-        take<TX, kMode, G>(held + off_x, x_rows + t * a.ldx, v, n, tid, width, x + v * (G / 2));
+        take<TX, kMode, G>(held + off_x, x_rows + t * a.ldx, v, c, x + v * (G / 2));
         if (kFull)
 #pragma unroll
           for (int j = 0; j < G / 2; ++j) ss = fma2(x[v * (G / 2) + j], x[v * (G / 2) + j], ss);
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
           if (p.r1 && tid == 0) p.r1[t] = r1;
         }
         if (left == 0) {
-          form_g1<TX, kVec, G>(a, ++group, g1, tid, width);
+          form_g1<TX, kVec, G>(a, ++group, g1, c);
           left = a.gate_rows;
         }
         --left;
@@ -108,10 +109,10 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
     for (int v = 0; v < kGroups; ++v) {
       float2* const hv = h + v * (G / 2);
       float2* const xv = x + v * (G / 2);
-      take<TR, kMode, G>(held, residual + t * a.ldr, v, n, tid, width, hv);
+      take<TR, kMode, G>(held, residual + t * a.ldr, v, c, hv);
       if constexpr (kFull) {
         float2 w[G / 2];
-        slots_load<G>(g1, v, tid, width, w);
+        slots_load<G>(g1, v, w);
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) hv[j] = fma2(both(a.scale), hv[j], mul2(mul2(xv[j], both(r1)), w[j]));
       } else if (a.x) {
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
       }
 #pragma unroll
       for (int j = 0; j < G / 2; ++j) ss = fma2(hv[j], hv[j], ss);
-      if (p.h) store_group<TR, kVec, G>(static_cast<TR*>(p.h) + t * n, v, n, tid, width, hv);
+      if (p.h) store_group<TR, kVec, G>(static_cast<TR*>(p.h) + t * n, v, c, hv);
     }
     if (a.gamma.ptr) {
       const float r2 = rsqrtf(row_sum(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
@@ -128,10 +129,10 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
 #pragma unroll
       for (int v = 0; v < kGroups; ++v) {
         float2 w[G / 2];
-        slots_load<G>(gammas, v, tid, width, w);
+        slots_load<G>(gammas, v, w);
 #pragma unroll
         for (int j = 0; j < G / 2; ++j) w[j] = mul2(mul2(h[v * (G / 2) + j], both(r2)), w[j]);
-        store_group<TX, kVec, G>(static_cast<TX*>(p.y) + t * n, v, n, tid, width, w);
+        store_group<TX, kVec, G>(static_cast<TX*>(p.y) + t * n, v, c, w);
       }
     }
   }
@@ -153,8 +154,7 @@ void forward_launch(NormParams& p, int threads, size_t smem, cudaStream_t stream
 template <typename TX, typename TR, bool kFull, int kMost>
 void forward_mode(NormParams& p, bool vec, int threads, cudaStream_t stream) {
   using Slots = ForwardSlots<TX, TR, kFull>;
-  const int n = p.a.hidden;
-  const RingSize size{threads, Slots::kWeights, Slots::kShare, window_bytes<TR>(n) + window_bytes<TX>(n)};
+  const RingSize size{threads, Slots::kWeights, Slots::kShare, window_bytes<TR>(threads) + window_bytes<TX>(threads)};
   size_t smem = 0;
   switch (choose_mode(size, vec, &p.ring, &smem)) {
     case kRing: forward_launch<TX, TR, kRing, kFull, kMost>(p, threads, smem, stream); break;
