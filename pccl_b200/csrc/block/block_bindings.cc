@@ -235,7 +235,7 @@ void check_move(const char* op, const Tensor& x, const Tensor& rows, const Tenso
   PCCL_ARG(offsets.dim() == 1 && offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.size(0) >= 1,
            op << ": routing.offsets must be contiguous int32 [experts + 1]");
   PCCL_ARG(rows.size(1) >= 1 && rows.numel() < INT_MAX, op << ": tokens * top_k must be below 2^31 and top_k at least 1");
-  PCCL_ARG(x.size(1) >= 1 && x.size(1) < INT_MAX / 2, op << ": rows hold at least one value");
+  PCCL_ARG(x.size(1) >= 1 && x.size(1) <= (1 << 24), op << ": rows hold at least one value and at most 2^24");
 }
 
 Tensor dispatch_run(const Tensor& x, const Tensor& rows, const Tensor& offsets) {

@@ -1,9 +1,13 @@
 // Rows of tokens into expert order and back: dispatch (one row to many), combine (weighted sum of many) and the
 // gradient of combine.  (The gradient of dispatch is combine without weights.)
 //
-// All three only move memory: a token's row is read once and kept in registers while its copies are written, or
-// its sources are read side by side and summed in 32 bits in the order of the choices, so the result does not
-// depend on the launch.  Row numbers outside the batch move nothing, whatever put them there.
+// All three only move memory: a token's row is read once for all its copies, or its sources are read side by side
+// and summed in 32 bits in the order of the choices, so the result does not depend on the launch.  Row numbers
+// outside the batch move nothing, whatever put them there.
+//
+// Work goes by chunks of 16 bytes of what is written.  Rows need not begin at 16 bytes (odd sizes, cut views): a
+// chunk's values then lie in two neighbouring 16-byte blocks of the source, which are loaded whole and shifted
+// together; only a row's first and last chunk go value by value.
 #include "../common/util.h"
 #include "../engine/cuda_driver.h"
 #include "vec.cuh"
@@ -25,34 +29,100 @@ struct MoveParams {
   float* dw;
 };
 
-// Eight values at element v of a row of `hidden`: 16 or 32 bytes at once, or one by one where rows are not aligned.
-template <typename T, bool kVec> __device__ __forceinline__ void load8(const T* row, int v, int hidden, float* f) {
-  if constexpr (kVec) {
-    unpack8<T>(load_raw8<T>(row + v), f);
-  } else {
+template <typename T> constexpr int kChunk = 16 / static_cast<int>(sizeof(T));
+
+template <typename T> __device__ __forceinline__ void unpack_chunk(uint4 q, float* f) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(row[min(v + i, hidden - 1)]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(w[i]);
+    else unpack2(w[i], f + 2 * i, T());
   }
 }
-template <typename T, bool kVec> __device__ __forceinline__ void store8(T* row, int v, int hidden, const float* f) {
-  if constexpr (kVec) {
-    store_raw8<T>(row + v, pack8<T>(f));
-  } else {
+template <typename T> __device__ __forceinline__ uint4 pack_chunk(const float* f) {
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (v + i < hidden) row[v + i] = from_f32<T>(f[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+    else w[i] = pack2(f[2 * i], f[2 * i + 1], T());
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// 16 bytes from any address: two neighbouring 16-byte blocks, and by how many bytes to shift them together.  Loading
+// and shifting are apart, and neither branches, so that several loads are under way at a time.
+struct Blocks {
+  uint4 lo, hi;
+  int off;
+};
+__device__ __forceinline__ uint4 shift_together(const Blocks& b) {
+  uint32_t w[8] = {b.lo.x, b.lo.y, b.lo.z, b.lo.w, b.hi.x, b.hi.y, b.hi.z, b.hi.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = b.off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = b.off & 4 ? w[i + 1] : w[i];
+  const int bits = (b.off & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+
+// The chunks of a row that is written: chunk i holds columns [first + i * N, + N), of which those inside the row count.
+// Aligned rows have first = 0 and whole chunks alone.
+template <typename T, bool kVec> struct RowChunks {
+  static constexpr int N = kChunk<T>;
+  int hidden, first, count;
+  __device__ RowChunks(const void* row, int hidden_) : hidden(hidden_) {
+    first = kVec ? 0 : -static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    count = (hidden - first + N - 1) / N;
+  }
+  __device__ int column(int i) const { return first + i * N; }
+  __device__ bool whole(int i) const { return kVec || (column(i) >= 0 && column(i) + N <= hidden); }
+  // A source row at chunk i.  Only blocks that hold a value of the row are read (allocations begin at multiples of 256
+  // bytes, so all of such a block is theirs): where one of the two does not, the other stands in for it, and what
+  // that brings lies outside the row.
+  __device__ Blocks load(const T* src, int i) const {
+    Blocks b;
+    const int c = column(i);
+    if constexpr (kVec) {
+      b.lo = __ldg(reinterpret_cast<const uint4*>(src + c));
+      b.hi = b.lo;
+      b.off = 0;
+    } else {
+      const uintptr_t row = reinterpret_cast<uintptr_t>(src), at = row + static_cast<int64_t>(c) * static_cast<int>(sizeof(T));
+      const uintptr_t begin = row & ~static_cast<uintptr_t>(15);
+      const uintptr_t end = (row + static_cast<uintptr_t>(hidden) * sizeof(T) - 1) & ~static_cast<uintptr_t>(15);
+      const uintptr_t lo = at & ~static_cast<uintptr_t>(15);
+      b.off = static_cast<int>(at & 15);
+      b.lo = __ldg(reinterpret_cast<const uint4*>(lo < begin ? begin : lo));
+      b.hi = __ldg(reinterpret_cast<const uint4*>(lo + 16 > end ? end : lo + 16));
+    }
+    return b;
+  }
+  __device__ static uint4 value(const Blocks& b) { return kVec ? b.lo : shift_together(b); }
+  __device__ void store(T* dst, int i, uint4 q) const {
+    const int c = column(i);
+    if (whole(i)) {
+      *reinterpret_cast<uint4*>(dst + c) = q;
+      return;
+    }
+    float f[N];
+    unpack_chunk<T>(q, f);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (c + j >= 0 && c + j < hidden) dst[c + j] = from_f32<T>(f[j]);
+  }
+};
 
 // Rows behind the last choice become zero.
 template <typename T, bool kVec> __device__ __forceinline__ void zero_tail(const MoveArgs& a, T* out) {
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
   int64_t used = a.offsets[a.experts];
   used = used < 0 ? 0 : used;
-  const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int64_t r = used + blockIdx.x; r < total; r += gridDim.x)
-    for (int v = threadIdx.x * 8; v < a.hidden; v += kThreads * 8)
-      store8<T, kVec>(out + r * a.hidden, v, a.hidden, zero);
+  for (int64_t r = used + blockIdx.x; r < total; r += gridDim.x) {
+    T* const dst = out + r * a.hidden;
+    const RowChunks<T, kVec> chunks(dst, a.hidden);
+    for (int i = threadIdx.x; i < chunks.count; i += kThreads) chunks.store(dst, i, make_uint4(0, 0, 0, 0));
+  }
 }
 
 template <typename T, bool kVec>
@@ -62,43 +132,77 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(const MoveParam
   T* out = static_cast<T*>(p.out);
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
     const T* src = static_cast<const T*>(p.x) + t * p.ldx;
-    for (int v = threadIdx.x * 8; v < a.hidden; v += kThreads * 8) {
-      float f[8];
-      load8<T, kVec>(src, v, a.hidden, f);
-      for (int k = 0; k < a.top_k; ++k) {
-        const int64_t r = a.rows[t * a.top_k + k];
-        if (r >= 0 && r < total) store8<T, kVec>(out + r * a.hidden, v, a.hidden, f);
+    const int32_t* rows = a.rows + t * a.top_k;
+    if constexpr (kVec) {
+      const RowChunks<T, true> chunks(src, a.hidden);
+      for (int i = threadIdx.x; i < chunks.count; i += kThreads) {
+        const uint4 q = chunks.value(chunks.load(src, i));
+        for (int k = 0; k < a.top_k; ++k) {
+          const int64_t r = rows[k];
+          if (r >= 0 && r < total) chunks.store(out + r * a.hidden, i, q);
+        }
+      }
+    } else {
+      for (int k = 0; k < a.top_k; ++k) {        // every copy has chunks of its own; the source stays in L1
+        const int64_t r = rows[k];
+        if (r < 0 || r >= total) continue;
+        T* const dst = out + r * a.hidden;
+        const RowChunks<T, false> chunks(dst, a.hidden);
+#pragma unroll 2
+        for (int i = threadIdx.x; i < chunks.count; i += kThreads) chunks.store(dst, i, chunks.value(chunks.load(src, i)));
       }
     }
   }
   zero_tail<T, kVec>(a, out);
 }
 
-template <typename T, bool kVec>
+// kAtOnce sources are under way at a time.
+template <typename T, bool kVec, int kAtOnce>
 __global__ void __launch_bounds__(kThreads) combine_rows_kernel(const MoveParams p) {
+  constexpr int N = kChunk<T>;
   const MoveArgs& a = p.a;
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
+  const T* y = static_cast<const T*>(p.x);
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    T* dst = static_cast<T*>(p.out) + t * a.hidden;
-    for (int v = threadIdx.x * 8; v < a.hidden; v += kThreads * 8) {
-      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < a.top_k; ++k) {
-        const int64_t r = a.rows[t * a.top_k + k];
-        if (r < 0 || r >= total) continue;
-        const float w = a.weights ? a.weights[t * a.top_k + k] : 1.f;
-        float f[8];
-        load8<T, kVec>(static_cast<const T*>(p.x) + r * p.ldx, v, a.hidden, f);
+    T* const dst = static_cast<T*>(p.out) + t * a.hidden;
+    const RowChunks<T, kVec> chunks(dst, a.hidden);
+    const int32_t* rows = a.rows + t * a.top_k;
+    const float* weights = a.weights ? a.weights + t * a.top_k : nullptr;
+    for (int i = threadIdx.x; i < chunks.count; i += kThreads) {
+      float acc[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+      for (int j = 0; j < N; ++j) acc[j] = 0.f;
+      for (int k0 = 0; k0 < a.top_k; k0 += kAtOnce) {
+        Blocks q[kAtOnce];
+        float w[kAtOnce];
+        bool valid[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int k = min(k0 + u, a.top_k - 1);
+          const int64_t r = rows[k];
+          valid[u] = k0 + u < a.top_k && r >= 0 && r < total;
+          w[u] = weights ? weights[k] : 1.f;
+          q[u] = chunks.load(y + (valid[u] ? r : 0) * p.ldx, i);       // row 0 is always there
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (valid[u]) {
+            float f[N];
+            unpack_chunk<T>(chunks.value(q[u]), f);
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = fmaf(w[u], f[j], acc[j]);
+          }
       }
-      store8<T, kVec>(dst, v, a.hidden, acc);
+      chunks.store(dst, i, pack_chunk<T>(acc));
     }
   }
 }
 
-// One warp per choice: its row of y and the token's dout pass through once for the product and the scaled copy.
+// One warp per choice: its row of y and the token's dout pass through once for the product and the scaled copy.  The
+// warps of a block take neighbouring choices, so a token's dout comes from L1 for all but the first.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) combine_rows_backward_kernel(const MoveParams p) {
+  constexpr int N = kChunk<T>, kAtOnce = kVec ? 4 : 2;
   const MoveArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
@@ -111,19 +215,37 @@ __global__ void __launch_bounds__(kThreads) combine_rows_backward_kernel(const M
       const float w = a.weights[i];
       const T* y = static_cast<const T*>(p.x) + r * p.ldx;
       const T* d = static_cast<const T*>(p.d) + i / a.top_k * p.ldd;
-      for (int v = lane * 8; v < a.hidden; v += 256) {
-        float fy[8], fd[8];
-        load8<T, kVec>(d, v, a.hidden, fd);
-        if (p.dw) {
-          load8<T, kVec>(y, v, a.hidden, fy);
+      T* const dst = out ? out + r * a.hidden : nullptr;
+      const RowChunks<T, kVec> chunks(dst ? static_cast<const void*>(dst) : y, a.hidden);
+      for (int c0 = lane; c0 < chunks.count; c0 += 32 * kAtOnce) {
+        Blocks qd[kAtOnce], qy[kAtOnce];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (kVec || v + j < a.hidden) dot = fmaf(fy[j], fd[j], dot);
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int c = min(c0 + 32 * u, chunks.count - 1);
+          qd[u] = chunks.load(d, c);
+          if (p.dw) qy[u] = chunks.load(y, c);
         }
-        if (out) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) fd[j] *= w;
-          store8<T, kVec>(out + r * a.hidden, v, a.hidden, fd);
+        for (int u = 0; u < kAtOnce; ++u) {
+          if (c0 + 32 * u >= chunks.count) break;
+          float fd[N], fy[N];
+          unpack_chunk<T>(chunks.value(qd[u]), fd);
+          if (p.dw) {
+            unpack_chunk<T>(chunks.value(qy[u]), fy);
+            if (!chunks.whole(c0 + 32 * u)) {
+              const int c = chunks.column(c0 + 32 * u);
+#pragma unroll
+              for (int j = 0; j < N; ++j)
+                if (c + j < 0 || c + j >= a.hidden) fd[j] = fy[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) dot = fmaf(fy[j], fd[j], dot);
+          }
+          if (dst) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) fd[j] *= w;
+            chunks.store(dst, c0 + 32 * u, pack_chunk<T>(fd));
+          }
         }
       }
     }
@@ -149,33 +271,41 @@ int grid_for(int64_t items) {
 
 }  // namespace
 
-#define PCCL_BLOCK_MOVE(KERNEL, ITEMS, VEC)                                                      \
+#define PCCL_BLOCK_MOVE(KERNEL, ITEMS, VEC, ...)                                                 \
   PCCL_BLOCK_TYPES(a.dtype, T,                                                                   \
-    if (VEC) KERNEL<T, true><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);                       \
-    else KERNEL<T, false><<<grid_for(ITEMS), kThreads, 0, stream>>>(p))                          \
+    if (VEC) KERNEL<T, true __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);           \
+    else KERNEL<T, false __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p))              \
   PCCL_CUDA(cudaGetLastError())
 
 void dispatch_rows(const MoveArgs& a, const void* x, int64_t ldx, void* out, cudaStream_t stream) {
-  if (a.tokens == 0 || a.hidden == 0) return;
+  if (a.tokens == 0) return;
   MoveParams p{a, x, ldx, nullptr, 0, out, nullptr};
-  const bool vec = a.hidden % 8 == 0 && aligned(x, ldx, a.dtype) && aligned(out, a.hidden, a.dtype);
-  PCCL_BLOCK_MOVE(dispatch_rows_kernel, a.tokens, vec);
+  const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(x, ldx, a.dtype) && aligned(out, a.hidden, a.dtype);
+  PCCL_BLOCK_MOVE(dispatch_rows_kernel, a.tokens, vec, );
 }
 
 void combine_rows(const MoveArgs& a, const void* y, int64_t ldy, void* out, cudaStream_t stream) {
-  if (a.tokens == 0 || a.hidden == 0) return;
+  if (a.tokens == 0) return;
   MoveParams p{a, y, ldy, nullptr, 0, out, nullptr};
-  const bool vec = a.hidden % 8 == 0 && aligned(y, ldy, a.dtype) && aligned(out, a.hidden, a.dtype);
-  PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec);
+  const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(y, ldy, a.dtype) && aligned(out, a.hidden, a.dtype);
+  // Up to four sources at a time, so many that the fewest loads go beyond the last one.
+  int at_once = a.top_k < 4 ? a.top_k : 4;
+  if (a.top_k > 4 && (a.top_k + 2) / 3 * 3 < (a.top_k + 3) / 4 * 4) at_once = 3;
+  switch (at_once) {
+    case 1: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 1); break;
+    case 2: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 2); break;
+    case 3: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 3); break;
+    default: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 4); break;
+  }
 }
 
 void combine_rows_backward(const MoveArgs& a, const void* y, int64_t ldy, const void* dout, int64_t ldd, void* dy,
                            float* dw, cudaStream_t stream) {
   if (a.tokens == 0 || (dy == nullptr && dw == nullptr)) return;
   MoveParams p{a, y, ldy, dout, ldd, dy, dw};
-  const bool vec = a.hidden % 8 == 0 && aligned(y, ldy, a.dtype) && aligned(dout, ldd, a.dtype) &&
+  const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(y, ldy, a.dtype) && aligned(dout, ldd, a.dtype) &&
                    (dy == nullptr || aligned(dy, a.hidden, a.dtype));
-  PCCL_BLOCK_MOVE(combine_rows_backward_kernel, static_cast<int64_t>(a.tokens) * a.top_k / 4, vec);
+  PCCL_BLOCK_MOVE(combine_rows_backward_kernel, (static_cast<int64_t>(a.tokens) * a.top_k + 7) / 8, vec, );
 }
 
 }  // namespace block

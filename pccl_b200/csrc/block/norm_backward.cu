@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
   const NormGrads& g = p.g;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
+  asm volatile("griddepcontrol.launch_dependents;");
   const Columns<kVec, G> c(n);
   row_sum_clear(sums);
   const int64_t begin = run_start(a.rows, p.workers, blockIdx.x), end = run_start(a.rows, p.workers, blockIdx.x + 1);
@@ -262,13 +263,16 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
   }
 }
 
-// Adds the workers' parts in their order: blockIdx.y 0 gamma, 1 post_gamma, 2.. the groups of gate rows.
-template <typename T>
-__global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormParams p) {
-  __shared__ float part[32][32];
+// Adds the blocks' parts in their order, a strip of them to each warp: blockIdx.y 0 gamma, 1 post_gamma, 2.. the
+// groups of gate rows.  C columns a thread (four where rows of parts are aligned).
+template <typename T, int C>
+__global__ void __launch_bounds__(512) norm_reduce_kernel(const NormParams p) {
+  struct alignas(C * 4) Part { float v[C]; };
+  __shared__ Part part[16][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const NormArgs& a = p.a;
   const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5, strips = blockDim.x >> 5, n = a.hidden;
-  const int col = blockIdx.x * 32 + lane;
+  const int col = (blockIdx.x * 32 + lane) * C;
   for (int64_t what = blockIdx.y; what < 2 + (p.part_gate ? a.rows / a.gate_rows : 0); what += gridDim.y) {
     const float* src;
     int first = 0, last = p.workers;
@@ -291,28 +295,51 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const NormParams p) {
       if (last - first == 1) src = nullptr;                  // written whole by its only worker
     }
     if (src == nullptr || out == nullptr) continue;
-    float sum = 0.f;
+    Part sum{};
+    const auto add = [&](const float* at) {
+      const Part q = *reinterpret_cast<const Part*>(at);
+#pragma unroll
+      for (int i = 0; i < C; ++i) sum.v[i] += q.v[i];
+    };
     if (col < n) {
       // Only the first of them can have begun with another group: its part stands in the second place.
-      if (strip == 0 && what >= 2) {
-        sum = src[first * step + (group * a.gate_rows > run_start(a.rows, p.workers, first) ? n : 0) + col];
-        ++first;
-      } else if (what >= 2) {
+      if (what >= 2) {
+        if (strip == 0) add(src + first * step + (group * a.gate_rows > run_start(a.rows, p.workers, first) ? n : 0) + col);
         ++first;
       }
       const float* at = src + (first + strip) * step + col;
 #pragma unroll 8
-      for (int w = first + strip; w < last; w += strips, at += strips * step) sum += *at;
+      for (int w = first + strip; w < last; w += strips, at += strips * step) add(at);
     }
     part[strip][lane] = sum;
     __syncthreads();
     if (strip == 0 && col < n) {
-for (int s = 1; s < strips; ++s) sum += part[s][lane];
-      if (f32) static_cast<float*>(out)[group * n + col] = sum;
-      else static_cast<T*>(out)[group * n + col] = from_f32<T>(sum);
+      for (int s = 1; s < strips; ++s)
+#pragma unroll
+        for (int i = 0; i < C; ++i) sum.v[i] += part[s][lane].v[i];
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (f32) static_cast<float*>(out)[group * n + col + i] = sum.v[i];
+        else static_cast<T*>(out)[group * n + col + i] = from_f32<T>(sum.v[i]);
+      }
     }
     __syncthreads();
   }
+}
+
+template <typename T, int C> void reduce_launch(const NormParams& p, cudaStream_t stream) {
+  // Its blocks may start while the first kernel ends; they wait for its results on the device.
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  const int64_t targets = 2 + (p.part_gate ? p.a.rows / p.a.gate_rows : 0);
+  config.gridDim = dim3((p.a.hidden + 32 * C - 1) / (32 * C), static_cast<unsigned>(targets < 1024 ? targets : 1024));
+  config.blockDim = dim3(512);
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  PCCL_CUDA(cudaLaunchKernelEx(&config, norm_reduce_kernel<T, C>, p));
 }
 
 // Blocks of the backward kernel: what an SM holds of them, each with at least one row.
@@ -374,11 +401,9 @@ void norm_backward(const NormArgs& a, const NormGrads& g, cudaStream_t stream) {
     else norm::backward_typed<T, float>(p, vec, stream))
   PCCL_CUDA(cudaGetLastError());
   if (g.dgamma || g.dpost_gamma || g.dgate) {
-    const int64_t targets = 2 + (g.dgate ? a.rows / a.gate_rows : 0);
-    const dim3 grid((a.hidden + 31) / 32, static_cast<unsigned>(targets < 1024 ? targets : 1024));
-    const int threads = p.workers > 512 ? 1024 : 256;      // strips of workers: short ones where there are many
-    PCCL_BLOCK_TYPES(a.xt, T, norm::norm_reduce_kernel<T><<<grid, threads, 0, stream>>>(p))
-    PCCL_CUDA(cudaGetLastError());
+    PCCL_BLOCK_TYPES(a.xt, T,
+      if (a.hidden % 4 == 0) norm::reduce_launch<T, 4>(p, stream);
+      else norm::reduce_launch<T, 1>(p, stream))
   }
 }
 

@@ -45,6 +45,7 @@ struct RouteParams {
   int tokens_per_block, words;
   int vec;                    // rows of logits can be read a lane's (or thread's) share at once
   int lanes;                  // lanes that share a group, a power of two; 0: groups do not divide so
+  uint32_t per_choice;        // 2^32 / top_k, rounded up: a choice's token without a division
 };
 
 // Unsigned keys in the order of the values; 0 stands below every value, infinities included.
@@ -365,7 +366,9 @@ __device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int 
 }
 
 // A lane's share of a row as it lies in memory.
-template <typename T, int NE> struct alignas(NE * sizeof(T) > 16 ? 16 : NE * sizeof(T)) Share { T v[NE]; };
+constexpr bool power_of_two(int n) { return (n & (n - 1)) == 0; }
+template <typename T, int NE>
+struct alignas(!power_of_two(NE) ? sizeof(T) : NE * sizeof(T) > 16 ? 16 : NE * sizeof(T)) Share { T v[NE]; };
 
 // Lanes and places beyond the last expert hold minus infinity: they have the highest numbers, so among equals every
 // expert comes before them, and there are always enough experts.
@@ -403,14 +406,15 @@ __device__ __forceinline__ float share_size(bool sigmoid_scores, float l, float 
   if (!sigmoid_scores) return expf(l - top);
   const float e = expf(-fabsf(l));
   const float up = l > 0.f ? 1.f : top > 0.f ? e : expf(l - top);
-  return up / (1.f + e);
+  return __fdividef(up, 1.f + e);                  // 2 ulp, of a divisor between 1 and 2
 }
 __device__ __forceinline__ float share(const RouteArgs& a, float l) {
   if (static_cast<int>(threadIdx.x & 31) >= a.top_k) l = -INFINITY;
-  const float top = warp_max(l);
+  float top = 1.f;                                 // for a sigmoid all that counts is whether one is positive
+  if (!a.sigmoid || !__any_sync(kAll, l > 0.f)) top = warp_max(l);
   if (top == -INFINITY) return 0.f;
   const float q = share_size(a.sigmoid, l, top);
-  return q / warp_sum(q);
+  return __fdividef(q, warp_sum(q));               // 2 ulp; the sum lies between 1/2 and top_k
 }
 
 // ---- rows in expert order --------------------------------------------------------------------------------------
@@ -449,17 +453,39 @@ __device__ __forceinline__ void block_scan(int32_t* value, int n, int32_t* part)
   __syncthreads();
 }
 
+// Shared memory of a block: marks [experts][words], marks ahead of each word [experts][words], choices
+// [tokens_per_block][top_k].
+struct BlockRows {
+  uint32_t* bits;
+  uint16_t* ahead;
+  uint16_t* chosen;
+  __device__ BlockRows(const RouteParams& p, uint32_t* smem) {
+    const int n = p.a.experts * p.words;
+    bits = smem;
+    ahead = reinterpret_cast<uint16_t*>(bits + n);
+    chosen = ahead + (n + 1) / 2 * 2;
+  }
+  __device__ void clear(const RouteParams& p) const {
+    for (int i = threadIdx.x; i < p.a.experts * p.words; i += blockDim.x) bits[i] = 0;
+  }
+  __device__ void mark(const RouteParams& p, int token, int e) const {
+    atomicOr(bits + e * p.words + (token >> 5), 1u << (token & 31));
+  }
+};
+
 // Counts and ranks of the block's marked choices.  With one block the rows are final; otherwise the counts go to
 // the second kernel, and the rows start at zero for every expert.
-__device__ __forceinline__ void finish_block(const RouteParams& p, const uint32_t* bits, const uint16_t* chosen,
-                                             int first, int count) {
+__device__ __forceinline__ void finish_block(const RouteParams& p, const BlockRows& b, int first, int count) {
   __shared__ int32_t base[kMaxExperts];
   __shared__ int32_t part[33];
   const RouteArgs& a = p.a;
   const bool alone = gridDim.x == 1;
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
     int n = 0;
-    for (int w = 0; w < p.words; ++w) n += __popc(bits[e * p.words + w]);
+    for (int w = 0; w < p.words; ++w) {
+      b.ahead[e * p.words + w] = static_cast<uint16_t>(n);
+      n += __popc(b.bits[e * p.words + w]);
+    }
     if (!alone) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + e] = static_cast<uint16_t>(n);
     base[e] = alone ? n : 0;
   }
@@ -470,14 +496,13 @@ __device__ __forceinline__ void finish_block(const RouteParams& p, const uint32_
     for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) a.offsets[e] = e < a.experts ? base[e] : part[32];
   }
   for (int i = threadIdx.x; i < count * a.top_k; i += blockDim.x) {
-    const int e = chosen[i], tok = i / a.top_k;
+    const int e = b.chosen[i], tok = a.top_k == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), p.per_choice));
     int row = -1;
     if (e != 0xffff) {
-      row = base[e];
-      for (int w = 0; w < tok >> 5; ++w) row += __popc(bits[e * p.words + w]);
-      row += __popc(bits[e * p.words + (tok >> 5)] & ((1u << (tok & 31)) - 1u));
+      const int at = e * p.words + (tok >> 5);
+      row = base[e] + b.ahead[at] + __popc(b.bits[at] & ((1u << (tok & 31)) - 1u));
     }
-    a.rows[static_cast<int64_t>(first) * a.top_k + i] = row;
+    a.rows[first * a.top_k + i] = row;
   }
 }
 
@@ -486,8 +511,7 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
   extern __shared__ uint32_t smem[];
   __shared__ uint16_t picks[kMost / 32][32];
   const RouteArgs& a = p.a;
-  uint32_t* bits = smem;                                             // [experts][words]
-  uint16_t* chosen = reinterpret_cast<uint16_t*>(bits + a.experts * p.words);   // [tokens_per_block][top_k]
+  const BlockRows mine(p, smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int first = blockIdx.x * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
@@ -499,7 +523,7 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
   float bias[NE];
 #pragma unroll
   for (int j = 0; j < NE; ++j) bias[j] = a.bias ? clean(a.bias[min(lane * NE + j, a.experts - 1)]) : 0.f;
-  for (int i = threadIdx.x; i < a.experts * p.words; i += blockDim.x) bits[i] = 0;
+  mine.clear(p);
   const bool grouped_sum = a.top2 && a.top_groups < a.groups;
   const bool scored = a.bias != nullptr || grouped_sum;              // the order needs the scores
   __syncthreads();
@@ -561,12 +585,12 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
       const int at = (first + i) * a.top_k + lane;
       a.idx[at] = e;
       a.weights[at] = w;
-      chosen[i * a.top_k + lane] = static_cast<uint16_t>(e);           // 0xffff: none
-      if (e >= 0) atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
+      mine.chosen[i * a.top_k + lane] = static_cast<uint16_t>(e);      // 0xffff: none
+      if (e >= 0) mine.mark(p, i, e);
     }
   }
   __syncthreads();
-  finish_block(p, bits, chosen, first, count);
+  finish_block(p, mine, first, count);
 }
 
 // ---- a thread per token ----------------------------------------------------------------------------------------
@@ -691,18 +715,17 @@ template <typename T, int NE>
 __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const RouteParams p) {
   extern __shared__ uint32_t smem[];
   const RouteArgs& a = p.a;
-  uint32_t* bits = smem;                                             // [experts][words]
-  uint16_t* chosen = reinterpret_cast<uint16_t*>(bits + a.experts * p.words);   // [tokens_per_block][top_k]
+  const BlockRows mine(p, smem);
   const int first = blockIdx.x * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
   asm volatile("griddepcontrol.launch_dependents;");
-  for (int i = threadIdx.x; i < a.experts * p.words; i += blockDim.x) bits[i] = 0;
+  mine.clear(p);
   const bool scored = a.bias != nullptr || (a.top2 && a.top_groups < a.groups);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += blockDim.x) {
     const int64_t t = first + i;
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-    uint16_t* const picked = chosen + i * a.top_k;
+    uint16_t* const picked = mine.chosen + i * a.top_k;
     const bool live = a.mask == nullptr || a.mask[t];
     float top = 0.f, total = 1.f;
     if (live) {
@@ -752,7 +775,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
         else if (a.sigmoid) w = sigmoid(le);
         else w = le == -INFINITY ? 0.f : expf(le - top) / total;
         w *= a.scale;
-        atomicOr(bits + e * p.words + (i >> 5), 1u << (i & 31));
+        mine.mark(p, i, e);
       } else {
         picked[k] = 0xffff;
       }
@@ -761,7 +784,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
     }
   }
   __syncthreads();
-  finish_block(p, bits, chosen, first, count);
+  finish_block(p, mine, first, count);
 }
 
 // Adds to every choice the rows of earlier experts and of earlier blocks of its own expert.  A thread sums two
@@ -951,15 +974,20 @@ __global__ void __launch_bounds__(128) route_thread_backward_kernel(const RouteP
 constexpr size_t kMaxRouteSmem = 96 * 1024;
 
 size_t route_smem(int experts, int top_k, int tokens_per_block) {
-  return static_cast<size_t>(experts) * (tokens_per_block / 32) * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2;
+  const size_t marks = static_cast<size_t>(experts) * (tokens_per_block / 32);
+  return marks * 4 + (marks + 1) / 2 * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2;
 }
 
 // Experts of a lane (or of a thread) that the kernels are compiled for.
 int share_of(int experts) {
   if (experts <= kThreadExperts) return experts <= 4 ? 4 : 8;
-  int ne = 1;
-  while (ne * 32 < experts) ne *= 2;
-  return ne;
+  const int ne = (experts + 31) / 32;
+  return ne <= 6 ? ne : ne <= 8 ? 8 : ne <= 16 ? 16 : 32;
+}
+// Lanes that share a group where a lane has `ne` experts, if groups fall into whole lanes, a power of two of them.
+int lanes_of(const RouteArgs& a, int ne) {
+  const int size = a.experts / a.groups;
+  return size % ne == 0 && power_of_two(size / ne) && a.groups * (size / ne) <= 32 ? size / ne : 0;
 }
 
 // Few tokens stay in one block, which needs no second kernel; more get about a block per SM.
@@ -1012,20 +1040,30 @@ void launch_threads(const RouteParams& p, bool backward, int blocks, size_t smem
 
 void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
   const RouteArgs& a = p.a;
-  const int ne = share_of(a.experts), bytes = dtype_bytes(a.dtype);
-  const int piece = ne * bytes < 16 ? ne * bytes : 16;
   const bool alone = a.experts <= kThreadExperts;
-  p.vec = (alone ? a.experts == ne : a.experts % ne == 0) && reinterpret_cast<uintptr_t>(a.logits) % piece == 0 &&
-          a.ld * bytes % piece == 0 &&
+  const int bytes = dtype_bytes(a.dtype);
+  int ne = share_of(a.experts);
+  p.lanes = lanes_of(a, ne);
+  // A few idle lanes are cheaper than groups that cross them.
+  if (!alone && a.top_groups < a.groups)
+    for (const int wider : {2, 3, 4, 5, 6, 8})
+      if (!p.lanes && wider > ne) {
+        p.lanes = lanes_of(a, wider);
+        if (p.lanes) ne = wider;
+      }
+  const int piece = ne * bytes < 16 ? ne * bytes : 16;
+  p.vec = power_of_two(ne) && (alone ? a.experts == ne : a.experts % ne == 0) &&
+          reinterpret_cast<uintptr_t>(a.logits) % piece == 0 && a.ld * bytes % piece == 0 &&
           (!backward || (reinterpret_cast<uintptr_t>(p.dlogits) % piece == 0 && static_cast<int64_t>(a.experts) * bytes % piece == 0));
-  const int size = a.experts / a.groups;
-  p.lanes = size % ne == 0 && ((size / ne) & (size / ne - 1)) == 0 && size / ne <= 32 ? size / ne : 0;
   PCCL_BLOCK_TYPES(a.dtype, T,
     if (alone && ne == 4) launch_threads<T, 4>(p, backward, blocks, smem, stream);
     else if (alone) launch_threads<T, 8>(p, backward, blocks, smem, stream);
     else if (ne == 1) launch_warps<T, 1>(p, backward, blocks, smem, stream);
     else if (ne == 2) launch_warps<T, 2>(p, backward, blocks, smem, stream);
+    else if (ne == 3) launch_warps<T, 3>(p, backward, blocks, smem, stream);
     else if (ne == 4) launch_warps<T, 4>(p, backward, blocks, smem, stream);
+    else if (ne == 5) launch_warps<T, 5>(p, backward, blocks, smem, stream);
+    else if (ne == 6) launch_warps<T, 6>(p, backward, blocks, smem, stream);
     else if (ne == 8) launch_warps<T, 8>(p, backward, blocks, smem, stream);
     else if (ne == 16) launch_warps<T, 16>(p, backward, blocks, smem, stream);
     else launch_warps<T, 32>(p, backward, blocks, smem, stream))
@@ -1046,6 +1084,7 @@ void route_topk(const RouteArgs& a, cudaStream_t stream) {
   p.tokens_per_block = tokens_per_block(a.tokens, a.experts, a.top_k);
   p.words = p.tokens_per_block / 32;
   p.pitch = (a.experts + 1) / 2 * 2;
+  p.per_choice = static_cast<uint32_t>((0x100000000ull + a.top_k - 1) / a.top_k);
   int blocks = (a.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks < 1) blocks = 1;
   p.counts = static_cast<uint16_t*>(a.workspace);
