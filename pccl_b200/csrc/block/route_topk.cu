@@ -45,6 +45,7 @@ struct RouteParams {
   int tokens_per_block, words;
   int vec;                    // rows of logits can be read a lane's (or thread's) share at once
   int lanes;                  // lanes that share a group, a power of two; 0: groups do not divide so
+  int block_words;            // 32-bit words of shared memory before the warps' decks
   uint32_t per_choice;        // 2^32 / top_k, rounded up: a choice's token without a division
 };
 
@@ -137,14 +138,25 @@ __device__ __forceinline__ int group_rank(int groups, int lanes, int group, Key 
   return rank;
 }
 
+// A warp's shared memory: the lanes' sorted keys, one above the other, and what was picked.
+template <int NE> struct Deck {
+  static constexpr int kKeys = NE <= 8 ? NE + 2 : 0;     // two rows of zeros below the last card
+  uint32_t key[kKeys > 0 ? kKeys : 1][32];
+  uint2 won[32];                                         // key, and lane * 8 + its lowest three bits
+  uint16_t picked[32];
+};
+
 // The choice in 32 bits with up to eight experts a lane.  The lowest three bits of a key give way to the expert's
 // place in the lane (lower places larger), so a lane's keys sort with two instructions a comparator and the number
 // comes with the key; lanes compare with those bits set.  That moves a score by less than 2^-20 of itself.  For
-// scores of 16 bits that no bias or sum has touched the bits carry nothing, and the choice is exact (kExact).
-// Results as for choose().
+// scores of 16 bits that no bias or sum has touched the bits carry nothing, and the choice is exact.
+//
+// A round finds the largest top card; its lane notes it and turns over the next one.  Selections, comparisons and
+// logic run at half the rate of other instructions and are what many tokens wait for, so the cards lie in shared memory
+// (shifting them in registers made a round cost 48 issue slots instead of 20).  Results as for choose().
 template <int NE>
 __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&s)[NE], float tau, bool exact, const float (&l)[NE],
-                                            uint16_t* picked) {
+                                            Deck<NE>& deck, int* pick) {
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   uint32_t key[NE];
@@ -152,6 +164,7 @@ __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&
   for (int j = 0; j < NE; ++j) key[j] = (key_of(s[j]) | 7u) ^ static_cast<uint32_t>(j);
   sort_lane<NE>(key);
   int close = 0;
+  bool kept = true;
   if (a.top_groups < a.groups) {                   // p.lanes neighbouring lanes a group
     uint32_t b1 = key[0] | 7u, b2 = NE > 1 ? key[NE > 1 ? 1 : 0] | 7u : 0u;
     for (int o = 1; o < p.lanes; o <<= 1) {
@@ -159,11 +172,11 @@ __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&
       b2 = larger(smaller(b1, o1), larger(b2, o2));
       b1 = larger(b1, o1);
     }
-    const int group = lane / p.lanes;
+    const int group = lane >> (__ffs(p.lanes) - 1);
     const uint32_t mine = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
     const bool real = group < a.groups;
     const int rank = group_rank(a.groups, p.lanes, group, mine);     // by the whole warp
-    const bool kept = real && rank < a.top_groups;
+    kept = real && rank < a.top_groups;
     if (!exact) {
       const float low = value_of(~warp_max(kept ? ~mine : 0u)), high = value_of(warp_max(real && !kept ? mine : 0u));
       if (!(low - high > 2.f * tau + 0x1p-18f * fabsf(low))) close = 2;
@@ -173,39 +186,43 @@ __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&
       for (int j = 0; j < NE; ++j) key[j] = (key_of(l[j]) | 7u) ^ static_cast<uint32_t>(j);
       sort_lane<NE>(key);
     }
-#pragma unroll
-    for (int j = 0; j < NE; ++j) key[j] = kept ? key[j] : 0u;
   }
-  uint32_t best = key[0] | 7u, won = 0;
+#pragma unroll
+  for (int j = 1; j < NE; ++j) deck.key[j][lane] = key[j];
+  const uint32_t* card = &deck.key[kept ? 0 : NE][lane];
+  uint32_t top = kept ? key[0] : 0u;
+  const unsigned below_me = (1u << lane) - 1u;
   const int rounds = a.top_k + (exact ? 0 : 1);
   for (int i = 0; i < rounds; ++i) {
-    const uint32_t m = warp_max(best);
-    won = lane == i ? m : won;
-    const bool own = lane == __ffs(__ballot_sync(kAll, best == m)) - 1;
-    if (own) picked[i] = static_cast<uint16_t>(lane * NE + (~key[0] & 7u));
-#pragma unroll
-    for (int j = 0; j + 1 < NE; ++j) key[j] = own ? key[j + 1] : key[j];
-    key[NE - 1] = own ? 0u : key[NE - 1];
-    best = key[0] | 7u;
+    const uint32_t best = top | 7u, m = warp_max(best);
+    const bool same = best == m;
+    const unsigned holders = __ballot_sync(kAll, same);
+    if (same && !(holders & below_me)) {
+      deck.won[i] = make_uint2(m, (top & 7u) | static_cast<uint32_t>(lane << 3));
+      card += 32;
+      top = *card;                                 // its own column: no other lane writes there
+    }
   }
   __syncwarp();
+  const uint2 won = deck.won[lane];
+  *pick = lane < rounds ? static_cast<int>(won.y >> 3) * NE + static_cast<int>(~won.y & 7u) : -1;
   if (!exact) {
-    const uint32_t below = __shfl_down_sync(kAll, won, 1);
+    const uint32_t below = __shfl_down_sync(kAll, won.x, 1);
     if (lane < a.top_k && below > 7u) {            // else there is no runner-up
-      const float score = value_of(won);
+      const float score = value_of(won.x);
       if (!(score - value_of(below) > tau + 0x1p-19f * fabsf(score) + 0x1p-140f)) close |= 1;
     }
   }
   return close;
 }
 
-// Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Expert
-// numbers go to picked[0 .. top_k - 1] in shared memory (with `check` the runner-up's behind them).  Returns whether
-// two scores that decide something differ by no more than tau (+ 2^-21 of their size): bit 0 in lane i for choices i and
-// i + 1, bit 1 for the groups.
+// Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Lane
+// i < top_k gets the i-th expert in *pick (with `check` lane top_k the runner-up).  Returns whether two scores that decide
+// something differ by no more than tau (+ 2^-21 of their size): bit 0 in lane i for choices i and i + 1, bit 1 for
+// the groups.
 template <typename F, int NE>
 __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], float tau, bool check, const float (&l)[NE],
-                                       uint16_t* picked) {
+                                       uint16_t* picked, int* pick) {
   using Key = decltype(key_of(F()));
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
@@ -303,6 +320,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
     }
   }
   __syncwarp();
+  *pick = lane < rounds ? static_cast<int>(picked[lane]) : -1;
   if (check) {
     const Key below = __shfl_down_sync(kAll, won, 1);
     if (lane < a.top_k && below != 0) {            // no runner-up: nothing to compare
@@ -313,23 +331,36 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
   return close;
 }
 
+// Calls f with copies: arrays whose address is taken live in memory, and these are needed in registers.
+template <int NE, class F>
+__device__ __forceinline__ int out_of_line(const float (&x)[NE], const float (&y)[NE], F f) {
+  float a[NE], b[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    a[j] = x[j];
+    b[j] = y[j];
+  }
+  return f(a, b);
+}
+
 // choose() out of line: groups that do not fall into whole lanes are rare, and should not cost the others registers.
 template <int NE>
 __device__ __noinline__ int choose_ragged(const RouteParams& p, const float (&s)[NE], float tau, bool check, const float (&l)[NE],
-                                          uint16_t* picked) {
-  return choose<float, NE>(p, s, tau, check, l, picked);
+                                          uint16_t* picked, int* pick) {
+  return choose<float, NE>(p, s, tau, check, l, picked, pick);
 }
 
 // The same choice from scores in 64 bits.
 template <int NE>
-__device__ __noinline__ void choose_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+__device__ __noinline__ int choose_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
   const RouteArgs& a = p.a;
+  int pick;
   double s[NE], total = 0;
   if (a.bias == nullptr && !(a.top2 && a.top_groups < a.groups)) {
 #pragma unroll
     for (int j = 0; j < NE; ++j) s[j] = static_cast<double>(l[j]);
-    choose<double, NE>(p, s, 0.f, false, l, picked);
-    return;
+    choose<double, NE>(p, s, 0.f, false, l, picked, &pick);
+    return pick;
   }
   float top = -INFINITY;
 #pragma unroll
@@ -347,17 +378,18 @@ __device__ __noinline__ void choose_wide(const RouteParams& p, const float (&l)[
     if (!a.sigmoid && total > 0) s[j] /= total;
     s[j] = l[j] == -INFINITY || bias[j] == -INFINITY ? -INFINITY : s[j] + static_cast<double>(bias[j]);
   }
-  choose<double, NE>(p, s, 0.f, false, l, picked);
+  choose<double, NE>(p, s, 0.f, false, l, picked, &pick);
+  return pick;
 }
 
 // Whether all that is close is a pair of choices with equal logits and equal biases, which no arithmetic can part.
 template <typename T>
-__device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, const uint16_t* picked) {
+__device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, int pick) {
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   float l = 0.f, b = 0.f;
   if (lane <= a.top_k && lane < a.experts) {
-    const int e = min(static_cast<int>(picked[lane]), a.experts - 1);
+    const int e = min(max(pick, 0), a.experts - 1);
     l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
     b = a.bias != nullptr ? a.bias[e] : 0.f;
   }
@@ -392,10 +424,22 @@ __device__ __forceinline__ void load_share(const RouteParams& p, int64_t t, Shar
       if (e0 + j < a.experts) to->v[j] = row[e0 + j];
   }
 }
+// Cleaned logits.  Products with zero show whether there is anything to clean, at a fifth of the cost of cleaning.
+// Returns whether this lane had an infinity or a NaN.
 template <typename T, int NE>
-__device__ __forceinline__ void clean_share(const Share<T, NE>& from, float (&l)[NE]) {
+__device__ __forceinline__ bool clean_share(const Share<T, NE>& from, float (&l)[NE]) {
+  float odd = 0.f;
 #pragma unroll
-  for (int j = 0; j < NE; ++j) l[j] = clean(to_f32<T>(from.v[j]));
+  for (int j = 0; j < NE; ++j) {
+    l[j] = to_f32<T>(from.v[j]) + 0.f;
+    odd = fmaf(l[j], 0.f, odd);
+  }
+  if (odd != 0.f) {                                // a NaN: from a NaN or an infinity
+#pragma unroll
+    for (int j = 0; j < NE; ++j) l[j] = clean(l[j]);
+    return true;
+  }
+  return false;
 }
 
 // Shares of the choices among themselves, sum 1 (0 where every chosen logit is -infinity).  Scaled by the
@@ -508,14 +552,14 @@ __device__ __forceinline__ void finish_block(const RouteParams& p, const BlockRo
 
 template <typename T, int NE, int kMost>
 __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams p) {
-  extern __shared__ uint32_t smem[];
-  __shared__ uint16_t picks[kMost / 32][32];
+  extern __shared__ __align__(16) uint32_t smem[];
   const RouteArgs& a = p.a;
   const BlockRows mine(p, smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int first = blockIdx.x * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
-  uint16_t* const picked = picks[warp];
+  Deck<NE>& deck = reinterpret_cast<Deck<NE>*>(smem + p.block_words)[warp];
+  uint16_t* const picked = deck.picked;
   asm volatile("griddepcontrol.launch_dependents;");
 
   Share<T, NE> next = empty_share<T, NE>();
@@ -524,6 +568,7 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
 #pragma unroll
   for (int j = 0; j < NE; ++j) bias[j] = a.bias ? clean(a.bias[min(lane * NE + j, a.experts - 1)]) : 0.f;
   mine.clear(p);
+  if constexpr (Deck<NE>::kKeys > 0) deck.key[NE][lane] = deck.key[NE + 1][lane] = 0;
   const bool grouped_sum = a.top2 && a.top_groups < a.groups;
   const bool scored = a.bias != nullptr || grouped_sum;              // the order needs the scores
   __syncthreads();
@@ -536,50 +581,66 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
     float w = 0.f;
     if (a.mask == nullptr || a.mask[t]) {
       float l[NE], s[NE];
-      clean_share<T, NE>(raw, l);
+      const bool odd = clean_share<T, NE>(raw, l);
       float top = 0.f, total = 1.f, tau = 0.f;
       if (!a.sigmoid && (scored || !a.renormalise)) {
         top = l[0];
 #pragma unroll
         for (int j = 1; j < NE; ++j) top = fmaxf(top, l[j]);
         top = warp_max(top);
+        if (top == -INFINITY) top = 0.f;                             // nothing is left: every exponential is zero
         total = 0.f;
+        if (a.renormalise) {
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          // The weights are made of these where they are not renormalised: then to the full 2^-22.
-          const float x = a.renormalise ? quick_exp(l[j] - top) : expf(l[j] - top);
-          s[j] = l[j] == -INFINITY ? 0.f : x;
-          total += s[j];
+          for (int j = 0; j < NE; ++j) total += s[j] = quick_exp(l[j] - top);
+        } else {
+          // The weights are made of these: to the full 2^-22.
+#pragma unroll
+          for (int j = 0; j < NE; ++j) total += s[j] = expf(l[j] - top);
         }
         total = warp_sum(total);
       }
       if (scored) {
         const float inv = total > 0.f ? 1.f / total : 0.f;
+        if (a.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < NE; ++j) {
-          const float prob = a.sigmoid ? quick_sigmoid(l[j]) : s[j] * inv;
-          s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
+          for (int j = 0; j < NE; ++j) s[j] = quick_sigmoid(l[j]) + bias[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < NE; ++j) s[j] = fmaf(s[j], inv, bias[j]);
+        }
+        if (odd) {                                                   // no bias brings back an expert that is out
+#pragma unroll
+          for (int j = 0; j < NE; ++j) s[j] = l[j] == -INFINITY ? -INFINITY : s[j];
         }
         tau = score_error(a.sigmoid, NE, inv);
       } else {
 #pragma unroll
         for (int j = 0; j < NE; ++j) s[j] = l[j];
       }
-      int close;
+      int close, pick;
       if constexpr (NE <= 8) {
-        if (a.top_groups == a.groups || p.lanes) close = choose_quick<NE>(p, s, tau, sizeof(T) == 2 && !scored, l, picked);
-        else close = choose_ragged<NE>(p, s, tau, scored, l, picked);
+        if (a.top_groups == a.groups || p.lanes) {
+          close = choose_quick<NE>(p, s, tau, sizeof(T) == 2 && !scored, l, deck, &pick);
+        } else {
+          int p1;
+          close = out_of_line(s, l, [&](const float (&s1)[NE], const float (&l1)[NE]) {
+            return choose_ragged<NE>(p, s1, tau, scored, l1, picked, &p1);
+          });
+          pick = p1;
+        }
       } else {
-        close = choose<float, NE>(p, s, tau, scored, l, picked);
+        close = choose<float, NE>(p, s, tau, scored, l, picked, &pick);
       }
-      if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, picked)) choose_wide<NE>(p, l, bias, picked);
-      e = lane < a.top_k ? picked[lane] : -1;
+      if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, pick))
+        pick = out_of_line(l, bias, [&](const float (&l1)[NE], const float (&b1)[NE]) { return choose_wide<NE>(p, l1, b1, picked); });
+      e = lane < a.top_k ? pick : -1;
       const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
       if (a.renormalise) w = share(a, le);
       else if (a.sigmoid) w = sigmoid(le);
       else w = le == -INFINITY ? 0.f : expf(le - top) / total;
       w *= a.scale;
-      __syncwarp();                                                  // picked is read
+      __syncwarp();                                                  // the deck is read
     }
     if (lane < a.top_k) {
       const int at = (first + i) * a.top_k + lane;
@@ -713,7 +774,7 @@ __device__ __forceinline__ void load_token(const RouteParams& p, int64_t t, floa
 
 template <typename T, int NE>
 __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const RouteParams p) {
-  extern __shared__ uint32_t smem[];
+  extern __shared__ __align__(16) uint32_t smem[];
   const RouteArgs& a = p.a;
   const BlockRows mine(p, smem);
   const int first = blockIdx.x * p.tokens_per_block;
@@ -755,7 +816,10 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
           s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
         }
         if (choose_alone<float, NE>(p, s, score_error(a.sigmoid, NE, inv), true, l, bias, picked))
-          choose_alone_wide<NE>(p, l, bias, picked);
+          out_of_line(l, bias, [&](const float (&l1)[NE], const float (&b1)[NE]) {
+            choose_alone_wide<NE>(p, l1, b1, picked);
+            return 0;
+          });
       } else {
         choose_alone<float, NE>(p, l, 0.f, false, l, bias, picked);
       }
@@ -975,7 +1039,7 @@ constexpr size_t kMaxRouteSmem = 96 * 1024;
 
 size_t route_smem(int experts, int top_k, int tokens_per_block) {
   const size_t marks = static_cast<size_t>(experts) * (tokens_per_block / 32);
-  return marks * 4 + (marks + 1) / 2 * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2;
+  return (marks * 4 + (marks + 1) / 2 * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2 + 15) / 16 * 16;
 }
 
 // Experts of a lane (or of a thread) that the kernels are compiled for.
@@ -1029,7 +1093,7 @@ void launch_warps(const RouteParams& p, bool backward, int blocks, size_t smem, 
   constexpr int kMost = NE <= 8 ? 1024 : 512;      // 64 or 128 registers a thread
   int threads = (p.a.tokens < p.tokens_per_block ? p.a.tokens : p.tokens_per_block) * 32;
   threads = threads < 128 ? 128 : threads > kMost ? kMost : threads;
-  launch_route(route_warp_kernel<T, NE, kMost>, p, blocks, threads, smem, stream);
+  launch_route(route_warp_kernel<T, NE, kMost>, p, blocks, threads, smem + threads / 32 * sizeof(Deck<NE>), stream);
 }
 
 template <typename T, int NE>
@@ -1087,6 +1151,7 @@ void route_topk(const RouteArgs& a, cudaStream_t stream) {
   p.per_choice = static_cast<uint32_t>((0x100000000ull + a.top_k - 1) / a.top_k);
   int blocks = (a.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks < 1) blocks = 1;
+  p.block_words = static_cast<int>(route_smem(a.experts, a.top_k, p.tokens_per_block) / 4);
   p.counts = static_cast<uint16_t*>(a.workspace);
   PCCL_CHECK(blocks == 1 || p.counts != nullptr, "route_topk: no workspace");
   launch_any(p, false, blocks, route_smem(a.experts, a.top_k, p.tokens_per_block), stream);
