@@ -99,6 +99,15 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
+// A tensor of 32-bit values in `storage`, from the offset-th on.
+Tensor slice_of(const c10::Storage& storage, at::IntArrayRef sizes, at::ScalarType type, int64_t offset) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                      c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && wants_grad(*t); }
 Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
@@ -137,16 +146,15 @@ variable_list route_run(const RouteCall& c, const Tensor& logits, const OptTenso
   const Tensor m = mask.has_value() ? mask->contiguous() : Tensor();
   if (b.defined()) a.bias = b.const_data_ptr<float>();
   if (m.defined()) a.mask = reinterpret_cast<const uint8_t*>(m.const_data_ptr<bool>());
-  Tensor idx = fresh({a.tokens, a.top_k}, at::kInt, logits);
-  Tensor weights = fresh({a.tokens, a.top_k}, at::kFloat, logits);
-  Tensor to = fresh({a.tokens, a.top_k}, at::kInt, logits);
-  Tensor offsets = fresh({a.experts + 1}, at::kInt, logits);
-  const size_t bytes = block::route_workspace(a.tokens, a.experts, a.top_k);
-  Tensor workspace;
-  if (bytes) {
-    workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, logits);
-    a.workspace = workspace.mutable_data_ptr();
-  }
+  // One allocation: an allocation costs the host as much as all of the arithmetic here costs the GPU for one token.
+  const int64_t n = static_cast<int64_t>(a.tokens) * a.top_k, rest = (3 * n + a.experts + 1 + 3) / 4 * 4;
+  const int64_t bytes = static_cast<int64_t>(block::route_workspace(a.tokens, a.experts, a.top_k));
+  const Tensor all = fresh({rest + (bytes + 3) / 4}, at::kInt, logits);
+  if (bytes) a.workspace = all.mutable_data_ptr<int32_t>() + rest;
+  Tensor idx = slice_of(all.storage(), {a.tokens, a.top_k}, at::kInt, 0);
+  Tensor weights = slice_of(all.storage(), {a.tokens, a.top_k}, at::kFloat, n);
+  Tensor to = slice_of(all.storage(), {a.tokens, a.top_k}, at::kInt, 2 * n);
+  Tensor offsets = slice_of(all.storage(), {a.experts + 1}, at::kInt, 3 * n);
   a.idx = idx.mutable_data_ptr<int32_t>();
   a.weights = weights.mutable_data_ptr<float>();
   a.rows = to.mutable_data_ptr<int32_t>();

@@ -41,7 +41,7 @@ struct RouteParams {
   const float* dweights;
   void* dlogits;
   uint16_t* counts;           // [blocks][pitch]: choices per expert of one block's tokens
-  int pitch;                  // experts, rounded up to even
+  int pitch;                  // experts, rounded up to a multiple of four
   int tokens_per_block, words;
   int vec;                    // rows of logits can be read a lane's (or thread's) share at once
   int lanes;                  // lanes that share a group, a power of two; 0: groups do not divide so
@@ -533,7 +533,8 @@ __device__ __forceinline__ void finish_block(const RouteParams& p, const BlockRo
     if (!alone) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + e] = static_cast<uint16_t>(n);
     base[e] = alone ? n : 0;
   }
-  if (!alone && threadIdx.x == 0 && (a.experts & 1)) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + a.experts] = 0;
+  if (!alone && a.experts + static_cast<int>(threadIdx.x) < p.pitch)
+    p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + a.experts + threadIdx.x] = 0;
   __syncthreads();
   if (alone) {
     block_scan(base, a.experts, part);
@@ -851,55 +852,61 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
   finish_block(p, mine, first, count);
 }
 
-// Adds to every choice the rows of earlier experts and of earlier blocks of its own expert.  A thread sums two
-// neighbouring experts over a strip of the blocks; whole numbers, so the order of the additions is free.
+// Adds to every choice the rows of earlier experts and of earlier blocks of its own expert.  A thread sums four
+// neighbouring experts over a strip of the blocks, all its loads under way at once; whole numbers, so the order of the
+// additions is free.
 __global__ void __launch_bounds__(kMostThreads, 1) route_rows_kernel(const RouteParams p) {
+  constexpr int kAtOnce = 10;                      // 148 blocks of 256 experts: 16 strips of 10
   const RouteArgs& a = p.a;
-  __shared__ int32_t before[kMaxExperts + 1], total[kMaxExperts + 1], part[33];
+  __shared__ int32_t before[kMaxExperts], total[kMaxExperts], part[33];
+  const int quads = p.pitch / 4, me = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
   for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) before[e] = total[e] = 0;
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int pairs = p.pitch / 2, me = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
   int width = 1;                                   // threads abreast: a power of two
-  while (width < pairs) width <<= 1;
+  while (width < quads) width <<= 1;
   const int strips = static_cast<int>(blockDim.x) / width, strip = threadIdx.x / width, col = threadIdx.x % width;
-  const uint32_t* counts = reinterpret_cast<const uint32_t*>(p.counts);
-  int b0 = 0, b1 = 0, t0 = 0, t1 = 0;
-  if (col < pairs) {
-#pragma unroll 8
-    for (int b = strip; b < blocks; b += strips) {
-      const uint32_t c = counts[static_cast<int64_t>(b) * pairs + col];
-      const int lo = c & 0xffffu, hi = c >> 16;
-      t0 += lo;
-      t1 += hi;
-      b0 += b < me ? lo : 0;
-      b1 += b < me ? hi : 0;
+  const uint2* counts = reinterpret_cast<const uint2*>(p.counts) + min(col, quads - 1);
+  int b[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
+  for (int b0 = strip; b0 < blocks; b0 += kAtOnce * strips) {
+    uint2 c[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) c[u] = counts[static_cast<int64_t>(min(b0 + u * strips, blocks - 1)) * quads];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int at = b0 + u * strips;
+      if (at >= blocks) break;
+      const int n[4] = {static_cast<int>(c[u].x & 0xffffu), static_cast<int>(c[u].x >> 16),
+                        static_cast<int>(c[u].y & 0xffffu), static_cast<int>(c[u].y >> 16)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        t[i] += n[i];
+        b[i] += at < me ? n[i] : 0;
+      }
     }
   }
-  for (int o = width; o < 32; o <<= 1) {           // lanes of the same column
-    b0 += __shfl_xor_sync(kAll, b0, o);
-    b1 += __shfl_xor_sync(kAll, b1, o);
-    t0 += __shfl_xor_sync(kAll, t0, o);
-    t1 += __shfl_xor_sync(kAll, t1, o);
-  }
-  if (col < pairs && (threadIdx.x & 31) < static_cast<unsigned>(width)) {
-    atomicAdd(before + 2 * col, b0);
-    atomicAdd(before + 2 * col + 1, b1);
-    atomicAdd(total + 2 * col, t0);
-    atomicAdd(total + 2 * col + 1, t1);
-  }
+  for (int o = width; o < 32; o <<= 1)             // lanes of the same column
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b[i] += __shfl_xor_sync(kAll, b[i], o);
+      t[i] += __shfl_xor_sync(kAll, t[i], o);
+    }
+  if (col < quads && (threadIdx.x & 31) < static_cast<unsigned>(width))
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      atomicAdd(before + 4 * col + i, b[i]);
+      atomicAdd(total + 4 * col + i, t[i]);
+    }
   __syncthreads();
   block_scan(total, a.experts, part);
   if (me == 0)
     for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) a.offsets[e] = e < a.experts ? total[e] : part[32];
-  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) before[e] += total[e];
-  __syncthreads();
   const int first = me * p.tokens_per_block;
   const int count = min(p.tokens_per_block, a.tokens - first);
   for (int i = threadIdx.x; i < count * a.top_k; i += blockDim.x) {
-    const int64_t at = static_cast<int64_t>(first) * a.top_k + i;
+    const int at = first * a.top_k + i;
     const int e = a.idx[at];
-    if (e >= 0) a.rows[at] += before[e];
+    if (e >= 0) a.rows[at] += before[e] + total[e];
   }
 }
 
@@ -1038,7 +1045,7 @@ __global__ void __launch_bounds__(128) route_thread_backward_kernel(const RouteP
 constexpr size_t kMaxRouteSmem = 96 * 1024;
 
 size_t route_smem(int experts, int top_k, int tokens_per_block) {
-  const size_t marks = static_cast<size_t>(experts) * (tokens_per_block / 32);
+  const size_t marks = static_cast<size_t>(experts) * ((tokens_per_block + 31) / 32);
   return (marks * 4 + (marks + 1) / 2 * 4 + static_cast<size_t>(tokens_per_block) * top_k * 2 + 15) / 16 * 16;
 }
 
@@ -1054,7 +1061,8 @@ int lanes_of(const RouteArgs& a, int ne) {
   return size % ne == 0 && power_of_two(size / ne) && a.groups * (size / ne) <= 32 ? size / ne : 0;
 }
 
-// Few tokens stay in one block, which needs no second kernel; more get about a block per SM.
+// Few tokens stay in one block, which needs no second kernel; more get about a block per SM, small ones as long as
+// there are SMs left (256 tokens of 256 experts: 32 a block 22.6 us, 8 a block 17).
 int tokens_per_block(int tokens, int experts, int top_k) {
   int tpb;
   if (experts <= kThreadExperts) {
@@ -1062,10 +1070,11 @@ int tokens_per_block(int tokens, int experts, int top_k) {
     if (tpb < 128 && tokens > 1024) tpb = 128;
     if (tpb > 1024) tpb = 1024;
   } else {
-    tpb = tokens <= 96 ? tokens : (tokens + 147) / 148;
+    tpb = tokens <= 24 ? tokens : (tokens + 147) / 148;
+    if (tpb < 8) tpb = 8;
   }
-  tpb = (tpb + 31) / 32 * 32;
-  if (tpb < 32) tpb = 32;
+  if (tpb > 32) tpb = (tpb + 31) / 32 * 32;
+  if (tpb < 1) tpb = 1;
   while (tpb > 32 && route_smem(experts, top_k, tpb) > kMaxRouteSmem) tpb -= 32;
   return tpb;
 }
@@ -1139,15 +1148,15 @@ void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStre
 size_t route_workspace(int tokens, int experts, int top_k) {
   const int tpb = tokens_per_block(tokens, experts, top_k);
   const int blocks = (tokens + tpb - 1) / tpb;
-  return blocks > 1 ? static_cast<size_t>(blocks) * ((experts + 1) / 2 * 2) * sizeof(uint16_t) : 0;
+  return blocks > 1 ? static_cast<size_t>(blocks) * ((experts + 3) / 4 * 4) * sizeof(uint16_t) : 0;
 }
 
 void route_topk(const RouteArgs& a, cudaStream_t stream) {
   RouteParams p{};
   p.a = a;
   p.tokens_per_block = tokens_per_block(a.tokens, a.experts, a.top_k);
-  p.words = p.tokens_per_block / 32;
-  p.pitch = (a.experts + 1) / 2 * 2;
+  p.words = (p.tokens_per_block + 31) / 32;
+  p.pitch = (a.experts + 3) / 4 * 4;
   p.per_choice = static_cast<uint32_t>((0x100000000ull + a.top_k - 1) / a.top_k);
   int blocks = (a.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks < 1) blocks = 1;
