@@ -97,11 +97,11 @@ __device__ __forceinline__ float quick_sigmoid(float l) {
 }
 
 // Bound of the difference of two scores' errors; quick_exp(x) is off by (2 + 1.2 |x|) 2^-23 of itself.  Sigmoid:
-// p (1 - p) times that is at most 0.7 * 2^-23, the sum and quotient add 2^-22.  Softmax: of the row's largest
+// p (1 - p) times that is at most 0.7 * 2^-23, the sum adds 2^-24 and the reciprocal 2^-23: 1.1 * 2^-21 for two.  Softmax: of the row's largest
 // probability, exponential 5 * 2^-24 (|x| e^-|x| < 0.37), the sum over a lane and the warp (n + 5) 2^-24 and its terms'
 // 5 * 2^-24, quotient and product 3 * 2^-24.
 __device__ __forceinline__ float score_error(bool sigmoid_scores, int n, float largest) {
-  return sigmoid_scores ? 0x1p-20f : static_cast<float>(n + 20) * 0x1p-23f * largest;
+  return sigmoid_scores ? 0x1.4p-21f : static_cast<float>(n + 20) * 0x1p-23f * largest;
 }
 
 // ---- a warp per token ------------------------------------------------------------------------------------------
@@ -138,6 +138,21 @@ __device__ __forceinline__ int group_rank(int groups, int lanes, int group, Key 
   return rank;
 }
 
+// Whether all that is close is a pair of choices with equal logits and equal biases, which no arithmetic can part.
+template <typename T>
+__device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, int pick) {
+  const RouteArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  float l = 0.f, b = 0.f;
+  if (lane <= a.top_k && lane < a.experts) {
+    const int e = min(max(pick, 0), a.experts - 1);
+    l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
+    b = a.bias != nullptr ? a.bias[e] : 0.f;
+  }
+  const float l1 = __shfl_down_sync(kAll, l, 1), b1 = __shfl_down_sync(kAll, b, 1);
+  return !__any_sync(kAll, (close & 2) || ((close & 1) && !(l == l1 && b == b1)));
+}
+
 // A warp's shared memory: the lanes' sorted keys, one above the other, and what was picked.
 template <int NE> struct Deck {
   static constexpr int kKeys = NE <= 8 ? NE + 2 : 0;     // two rows of zeros below the last card
@@ -153,18 +168,21 @@ template <int NE> struct Deck {
 //
 // A round finds the largest top card; its lane notes it and turns over the next one.  Selections, comparisons and
 // logic run at half the rate of other instructions and are what many tokens wait for, so the cards lie in shared memory
-// (shifting them in registers made a round cost 48 issue slots instead of 20).  Results as for choose().
-template <int NE>
-__device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&s)[NE], float tau, bool exact, const float (&l)[NE],
-                                            Deck<NE>& deck, int* pick) {
+// (a round of 65536 tokens took 3.7 us with the keys shifted in registers, 2.7 so).
+//
+// Where neighbours of the choice are close, the choices and the runner-up are ranked again by 64-bit scores, a lane
+// each: enough unless something behind the runner-up is close to it as well, is not its equal in logit and bias, or
+// the scores need the whole row's sum.  Returns whether the choice has to be repeated over all experts.
+template <typename T, int NE>
+__device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, const float (&s)[NE], float tau, bool exact,
+                                             const float (&l)[NE], const float (&bias)[NE], Deck<NE>& deck, int* pick) {
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   uint32_t key[NE];
 #pragma unroll
   for (int j = 0; j < NE; ++j) key[j] = (key_of(s[j]) | 7u) ^ static_cast<uint32_t>(j);
   sort_lane<NE>(key);
-  int close = 0;
-  bool kept = true;
+  bool again = false, kept = true;
   if (a.top_groups < a.groups) {                   // p.lanes neighbouring lanes a group
     uint32_t b1 = key[0] | 7u, b2 = NE > 1 ? key[NE > 1 ? 1 : 0] | 7u : 0u;
     for (int o = 1; o < p.lanes; o <<= 1) {
@@ -179,7 +197,8 @@ __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&
     kept = real && rank < a.top_groups;
     if (!exact) {
       const float low = value_of(~warp_max(kept ? ~mine : 0u)), high = value_of(warp_max(real && !kept ? mine : 0u));
-      if (!(low - high > 2.f * tau + 0x1p-18f * fabsf(low))) close = 2;
+      // Two scores each, whose keys lose up to seven units in one direction.
+      again = !(low - high > 2.f * tau + 0x1.4p-20f * fabsf(low) + 0x1p-140f);
     }
     if (a.top2 && a.bias == nullptr) {             // the groups by their sums, the experts by their logits
 #pragma unroll
@@ -205,15 +224,50 @@ __device__ __forceinline__ int choose_quick(const RouteParams& p, const float (&
   }
   __syncwarp();
   const uint2 won = deck.won[lane];
-  *pick = lane < rounds ? static_cast<int>(won.y >> 3) * NE + static_cast<int>(~won.y & 7u) : -1;
-  if (!exact) {
-    const uint32_t below = __shfl_down_sync(kAll, won.x, 1);
-    if (lane < a.top_k && below > 7u) {            // else there is no runner-up
-      const float score = value_of(won.x);
-      if (!(score - value_of(below) > tau + 0x1p-19f * fabsf(score) + 0x1p-140f)) close |= 1;
-    }
+  const bool there = lane < rounds && won.x > 7u;            // a runner-up can be missing
+  *pick = there ? static_cast<int>(won.y >> 3) * NE + static_cast<int>(~won.y & 7u) : -1;
+  if (exact) return false;
+  if (a.bias == nullptr) tau = 0.f;                          // ranked by logits
+  // Scores nearer than this may stand the other way round.  (Keys lose up to seven units, all in one direction.)
+  const auto reach = [&](float score) { return tau + 0x1.4p-20f * fabsf(score) + 0x1p-140f; };
+  const uint32_t below = __shfl_down_sync(kAll, won.x, 1);
+  const float score = value_of(won.x);
+  const bool close = lane < a.top_k && below > 7u && !(score - value_of(below) > reach(score));
+  if (again || !__any_sync(kAll, close)) return again;
+  if (a.bias != nullptr && !a.sigmoid) return !truly_tied<T>(p, t, close ? 1 : 0, *pick);
+
+  float le = 0.f, be = 0.f;
+  if (there) {
+    le = clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + *pick]));
+    be = a.bias ? clean(a.bias[*pick]) : 0.f;
   }
-  return close;
+  const uint32_t next = warp_max(top | 7u), last = __shfl_sync(kAll, won.x, a.top_k);
+  const float edge = value_of(last);
+  if (last > 7u && next > 7u && !(edge - value_of(next) > reach(edge))) {
+    // Something behind the runner-up is close to it.  Only its equals may be: all that reaches it and is not its
+    // equal has to be among the choices.
+    const float lr = __shfl_sync(kAll, le, a.top_k), br = __shfl_sync(kAll, be, a.top_k);
+    int others = 0;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      const float v = a.bias ? s[j] : l[j];
+      others += __popc(__ballot_sync(kAll, kept && !(edge - v > 2.f * reach(edge)) && !(l[j] == lr && (!a.bias || bias[j] == br))));
+    }
+    const unsigned chosen = __ballot_sync(kAll, lane < a.top_k && !(le == lr && be == br));
+    if (others != __popc(chosen)) return true;
+  }
+  double wide = a.bias == nullptr ? static_cast<double>(le) : 1.0 / (1.0 + exp(-static_cast<double>(le))) + static_cast<double>(be);
+  if (le == -INFINITY || be == -INFINITY || !there) wide = -INFINITY;
+  int rank = 0;
+  for (int i = 0; i < rounds; ++i) {
+    const double other = __shfl_sync(kAll, wide, i);
+    const int e = __shfl_sync(kAll, *pick, i);
+    if (e >= 0) rank += other > wide || (other == wide && e < *pick) ? 1 : 0;
+  }
+  if (there) deck.picked[rank] = static_cast<uint16_t>(*pick);
+  __syncwarp();
+  if (there) *pick = deck.picked[lane];
+  return false;
 }
 
 // Choice of one token by scores s[NE]; without a bias they rank the groups and the logits rank the experts.  Lane
@@ -380,21 +434,6 @@ __device__ __noinline__ int choose_wide(const RouteParams& p, const float (&l)[N
   }
   choose<double, NE>(p, s, 0.f, false, l, picked, &pick);
   return pick;
-}
-
-// Whether all that is close is a pair of choices with equal logits and equal biases, which no arithmetic can part.
-template <typename T>
-__device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, int pick) {
-  const RouteArgs& a = p.a;
-  const int lane = threadIdx.x & 31;
-  float l = 0.f, b = 0.f;
-  if (lane <= a.top_k && lane < a.experts) {
-    const int e = min(max(pick, 0), a.experts - 1);
-    l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
-    b = a.bias != nullptr ? a.bias[e] : 0.f;
-  }
-  const float l1 = __shfl_down_sync(kAll, l, 1), b1 = __shfl_down_sync(kAll, b, 1);
-  return !__any_sync(kAll, (close & 2) || ((close & 1) && !(l == l1 && b == b1)));
 }
 
 // A lane's share of a row as it lies in memory.
@@ -619,21 +658,24 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
 #pragma unroll
         for (int j = 0; j < NE; ++j) s[j] = l[j];
       }
-      int close, pick;
+      int pick;
+      bool again;
       if constexpr (NE <= 8) {
         if (a.top_groups == a.groups || p.lanes) {
-          close = choose_quick<NE>(p, s, tau, sizeof(T) == 2 && !scored, l, deck, &pick);
+          again = choose_quick<T, NE>(p, t, s, tau, sizeof(T) == 2 && !scored, l, bias, deck, &pick);
         } else {
           int p1;
-          close = out_of_line(s, l, [&](const float (&s1)[NE], const float (&l1)[NE]) {
+          const int close = out_of_line(s, l, [&](const float (&s1)[NE], const float (&l1)[NE]) {
             return choose_ragged<NE>(p, s1, tau, scored, l1, picked, &p1);
           });
           pick = p1;
+          again = __any_sync(kAll, close) && !truly_tied<T>(p, t, close, pick);
         }
       } else {
-        close = choose<float, NE>(p, s, tau, scored, l, picked, &pick);
+        const int close = choose<float, NE>(p, s, tau, scored, l, picked, &pick);
+        again = __any_sync(kAll, close) && !truly_tied<T>(p, t, close, pick);
       }
-      if (__any_sync(kAll, close) && !truly_tied<T>(p, t, close, pick))
+      if (again)
         pick = out_of_line(l, bias, [&](const float (&l1)[NE], const float (&b1)[NE]) { return choose_wide<NE>(p, l1, b1, picked); });
       e = lane < a.top_k ? pick : -1;
       const float le = e >= 0 ? clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e])) : -INFINITY;
