@@ -17,7 +17,7 @@ namespace block {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kFull = 8;          // a block, and how many times two that is
 
 struct MoveParams {
   MoveArgs a;
@@ -27,6 +27,7 @@ struct MoveParams {
   int64_t ldd;
   void* out;
   float* dw;
+  int shift;                  // 1 << shift threads share a row (kFull: all of a block, known when compiled)
 };
 
 template <typename T> constexpr int kChunk = 16 / static_cast<int>(sizeof(T));
@@ -114,28 +115,33 @@ template <typename T, bool kVec> struct RowChunks {
 };
 
 // Rows behind the last choice become zero.
-template <typename T, bool kVec> __device__ __forceinline__ void zero_tail(const MoveArgs& a, T* out) {
+template <typename T, bool kVec> __device__ __forceinline__ void zero_tail(const MoveArgs& a, T* out, const int shift) {
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
   int64_t used = a.offsets[a.experts];
   used = used < 0 ? 0 : used;
-  for (int64_t r = used + blockIdx.x; r < total; r += gridDim.x) {
+  const int lanes = 1 << shift, rows = kThreads >> shift;
+  for (int64_t r = used + static_cast<int64_t>(blockIdx.x) * rows + (threadIdx.x >> shift); r < total;
+       r += static_cast<int64_t>(gridDim.x) * rows) {
     T* const dst = out + r * a.hidden;
     const RowChunks<T, kVec> chunks(dst, a.hidden);
-    for (int i = threadIdx.x; i < chunks.count; i += kThreads) chunks.store(dst, i, make_uint4(0, 0, 0, 0));
+    for (int i = threadIdx.x & (lanes - 1); i < chunks.count; i += lanes) chunks.store(dst, i, make_uint4(0, 0, 0, 0));
   }
 }
 
-template <typename T, bool kVec>
+template <typename T, bool kVec, bool kLong>
 __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(const MoveParams p) {
   const MoveArgs& a = p.a;
+  const int shift = kLong ? kFull : p.shift;
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
   T* out = static_cast<T*>(p.out);
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  const int lanes = 1 << shift, rows_abreast = kThreads >> shift, tid = threadIdx.x & (lanes - 1);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * rows_abreast + (threadIdx.x >> shift); t < a.tokens;
+       t += static_cast<int64_t>(gridDim.x) * rows_abreast) {
     const T* src = static_cast<const T*>(p.x) + t * p.ldx;
     const int32_t* rows = a.rows + t * a.top_k;
     if constexpr (kVec) {
       const RowChunks<T, true> chunks(src, a.hidden);
-      for (int i = threadIdx.x; i < chunks.count; i += kThreads) {
+      for (int i = tid; i < chunks.count; i += lanes) {
         const uint4 q = chunks.value(chunks.load(src, i));
         for (int k = 0; k < a.top_k; ++k) {
           const int64_t r = rows[k];
@@ -149,26 +155,29 @@ __global__ void __launch_bounds__(kThreads) dispatch_rows_kernel(const MoveParam
         T* const dst = out + r * a.hidden;
         const RowChunks<T, false> chunks(dst, a.hidden);
 #pragma unroll 2
-        for (int i = threadIdx.x; i < chunks.count; i += kThreads) chunks.store(dst, i, chunks.value(chunks.load(src, i)));
+        for (int i = tid; i < chunks.count; i += lanes) chunks.store(dst, i, chunks.value(chunks.load(src, i)));
       }
     }
   }
-  zero_tail<T, kVec>(a, out);
+  zero_tail<T, kVec>(a, out, shift);
 }
 
 // kAtOnce sources are under way at a time.
-template <typename T, bool kVec, int kAtOnce>
+template <typename T, bool kVec, bool kLong, int kAtOnce>
 __global__ void __launch_bounds__(kThreads) combine_rows_kernel(const MoveParams p) {
   constexpr int N = kChunk<T>;
   const MoveArgs& a = p.a;
+  const int shift = kLong ? kFull : p.shift;
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
   const T* y = static_cast<const T*>(p.x);
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  const int lanes = 1 << shift, rows_abreast = kThreads >> shift, tid = threadIdx.x & (lanes - 1);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * rows_abreast + (threadIdx.x >> shift); t < a.tokens;
+       t += static_cast<int64_t>(gridDim.x) * rows_abreast) {
     T* const dst = static_cast<T*>(p.out) + t * a.hidden;
     const RowChunks<T, kVec> chunks(dst, a.hidden);
     const int32_t* rows = a.rows + t * a.top_k;
     const float* weights = a.weights ? a.weights + t * a.top_k : nullptr;
-    for (int i = threadIdx.x; i < chunks.count; i += kThreads) {
+    for (int i = tid; i < chunks.count; i += lanes) {
       float acc[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = 0.f;
@@ -198,18 +207,20 @@ __global__ void __launch_bounds__(kThreads) combine_rows_kernel(const MoveParams
   }
 }
 
-// One warp per choice: its row of y and the token's dout pass through once for the product and the scaled copy.  The
+// One warp (of short rows: part of one) per choice: its row of y and the token's dout pass through once for the product and the scaled copy.  The
 // warps of a block take neighbouring choices, so a token's dout comes from L1 for all but the first.
-template <typename T, bool kVec>
+template <typename T, bool kVec, bool kLong>
 __global__ void __launch_bounds__(kThreads) combine_rows_backward_kernel(const MoveParams p) {
   constexpr int N = kChunk<T>, kAtOnce = kVec ? 4 : 2;
   const MoveArgs& a = p.a;
-  const int lane = threadIdx.x & 31;
+  const int shift = kLong || p.shift > 5 ? 5 : p.shift, width = 1 << shift, lane = threadIdx.x & (width - 1);
   const int64_t total = static_cast<int64_t>(a.tokens) * a.top_k;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  const int64_t abreast = static_cast<int64_t>(gridDim.x) * (kThreads >> shift);
   T* out = static_cast<T*>(p.out);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); i < total; i += warps) {
-    const int64_t r = a.rows[i];
+  // Whole warps go round together: the sum at the end is by all of their lanes.
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kThreads >> shift); i0 < total; i0 += abreast) {
+    const int64_t i = i0 + (threadIdx.x >> shift);
+    const int64_t r = i < total ? a.rows[i] : -1;
     float dot = 0.f;
     if (r >= 0 && r < total) {
       const float w = a.weights[i];
@@ -217,23 +228,23 @@ __global__ void __launch_bounds__(kThreads) combine_rows_backward_kernel(const M
       const T* d = static_cast<const T*>(p.d) + i / a.top_k * p.ldd;
       T* const dst = out ? out + r * a.hidden : nullptr;
       const RowChunks<T, kVec> chunks(dst ? static_cast<const void*>(dst) : y, a.hidden);
-      for (int c0 = lane; c0 < chunks.count; c0 += 32 * kAtOnce) {
+      for (int c0 = lane; c0 < chunks.count; c0 += width * kAtOnce) {
         Blocks qd[kAtOnce], qy[kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-          const int c = min(c0 + 32 * u, chunks.count - 1);
+          const int c = min(c0 + width * u, chunks.count - 1);
           qd[u] = chunks.load(d, c);
           if (p.dw) qy[u] = chunks.load(y, c);
         }
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-          if (c0 + 32 * u >= chunks.count) break;
+          if (c0 + width * u >= chunks.count) break;
           float fd[N], fy[N];
           unpack_chunk<T>(chunks.value(qd[u]), fd);
           if (p.dw) {
             unpack_chunk<T>(chunks.value(qy[u]), fy);
-            if (!chunks.whole(c0 + 32 * u)) {
-              const int c = chunks.column(c0 + 32 * u);
+            if (!chunks.whole(c0 + width * u)) {
+              const int c = chunks.column(c0 + width * u);
 #pragma unroll
               for (int j = 0; j < N; ++j)
                 if (c + j < 0 || c + j >= a.hidden) fd[j] = fy[j] = 0.f;
@@ -244,17 +255,17 @@ __global__ void __launch_bounds__(kThreads) combine_rows_backward_kernel(const M
           if (dst) {
 #pragma unroll
             for (int j = 0; j < N; ++j) fd[j] *= w;
-            chunks.store(dst, c0 + 32 * u, pack_chunk<T>(fd));
+            chunks.store(dst, c0 + width * u, pack_chunk<T>(fd));
           }
         }
       }
     }
     if (p.dw) {
-      dot = warp_sum(dot);
-      if (lane == 0) p.dw[i] = dot;
+      for (int o = width / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane == 0 && i < total) p.dw[i] = dot;
     }
   }
-  if (out) zero_tail<T, kVec>(a, out);
+  if (out) zero_tail<T, kVec>(a, out, kLong ? kFull : p.shift);
 }
 
 bool aligned(const void* p, int64_t ld, DType t) {
@@ -269,43 +280,57 @@ int grid_for(int64_t items) {
   return static_cast<int>(items < 1 ? 1 : items < most ? items : most);
 }
 
+// As many threads as a row has chunks (one more where it begins inside one), four at least.
+int shift_for(const MoveArgs& a) {
+  const int chunks = (a.hidden * dtype_bytes(a.dtype) + 15) / 16 + (a.hidden * dtype_bytes(a.dtype) % 16 ? 1 : 0);
+  int shift = 2;
+  while ((1 << shift) < chunks && (1 << shift) < kThreads) ++shift;
+  return shift;
+}
+
 }  // namespace
 
 #define PCCL_BLOCK_MOVE(KERNEL, ITEMS, VEC, ...)                                                 \
   PCCL_BLOCK_TYPES(a.dtype, T,                                                                   \
-    if (VEC) KERNEL<T, true __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);           \
-    else KERNEL<T, false __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p))              \
+    if (VEC && p.shift == kFull) KERNEL<T, true, true __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);   \
+    else if (VEC) KERNEL<T, true, false __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);                 \
+    else if (p.shift == kFull) KERNEL<T, false, true __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p);    \
+    else KERNEL<T, false, false __VA_ARGS__><<<grid_for(ITEMS), kThreads, 0, stream>>>(p))                         \
   PCCL_CUDA(cudaGetLastError())
 
 void dispatch_rows(const MoveArgs& a, const void* x, int64_t ldx, void* out, cudaStream_t stream) {
   if (a.tokens == 0) return;
-  MoveParams p{a, x, ldx, nullptr, 0, out, nullptr};
+  MoveParams p{a, x, ldx, nullptr, 0, out, nullptr, shift_for(a)};
+  const int64_t blocks = ((static_cast<int64_t>(a.tokens) << p.shift) + kThreads - 1) / kThreads;
   const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(x, ldx, a.dtype) && aligned(out, a.hidden, a.dtype);
-  PCCL_BLOCK_MOVE(dispatch_rows_kernel, a.tokens, vec, );
+  PCCL_BLOCK_MOVE(dispatch_rows_kernel, blocks, vec, );
 }
 
 void combine_rows(const MoveArgs& a, const void* y, int64_t ldy, void* out, cudaStream_t stream) {
   if (a.tokens == 0) return;
-  MoveParams p{a, y, ldy, nullptr, 0, out, nullptr};
+  MoveParams p{a, y, ldy, nullptr, 0, out, nullptr, shift_for(a)};
+  const int64_t blocks = ((static_cast<int64_t>(a.tokens) << p.shift) + kThreads - 1) / kThreads;
   const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(y, ldy, a.dtype) && aligned(out, a.hidden, a.dtype);
   // Up to four sources at a time, so many that the fewest loads go beyond the last one.
   int at_once = a.top_k < 4 ? a.top_k : 4;
   if (a.top_k > 4 && (a.top_k + 2) / 3 * 3 < (a.top_k + 3) / 4 * 4) at_once = 3;
   switch (at_once) {
-    case 1: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 1); break;
-    case 2: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 2); break;
-    case 3: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 3); break;
-    default: PCCL_BLOCK_MOVE(combine_rows_kernel, a.tokens, vec, , 4); break;
+    case 1: PCCL_BLOCK_MOVE(combine_rows_kernel, blocks, vec, , 1); break;
+    case 2: PCCL_BLOCK_MOVE(combine_rows_kernel, blocks, vec, , 2); break;
+    case 3: PCCL_BLOCK_MOVE(combine_rows_kernel, blocks, vec, , 3); break;
+    default: PCCL_BLOCK_MOVE(combine_rows_kernel, blocks, vec, , 4); break;
   }
 }
 
 void combine_rows_backward(const MoveArgs& a, const void* y, int64_t ldy, const void* dout, int64_t ldd, void* dy,
                            float* dw, cudaStream_t stream) {
   if (a.tokens == 0 || (dy == nullptr && dw == nullptr)) return;
-  MoveParams p{a, y, ldy, dout, ldd, dy, dw};
+  MoveParams p{a, y, ldy, dout, ldd, dy, dw, shift_for(a)};
+  const int shift = p.shift < 5 ? p.shift : 5;
+  const int64_t blocks = ((static_cast<int64_t>(a.tokens) * a.top_k << shift) + kThreads - 1) / kThreads;
   const bool vec = a.hidden * dtype_bytes(a.dtype) % 16 == 0 && aligned(y, ldy, a.dtype) && aligned(dout, ldd, a.dtype) &&
                    (dy == nullptr || aligned(dy, a.hidden, a.dtype));
-  PCCL_BLOCK_MOVE(combine_rows_backward_kernel, (static_cast<int64_t>(a.tokens) * a.top_k + 7) / 8, vec, );
+  PCCL_BLOCK_MOVE(combine_rows_backward_kernel, blocks, vec, );
 }
 
 }  // namespace block

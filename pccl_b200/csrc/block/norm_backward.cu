@@ -11,6 +11,8 @@
 //
 // A block takes a run of consecutive rows and sums the weights' gradients in registers; a second kernel adds the
 // blocks' sums in their order, so results do not depend on timing.
+#include <type_traits>
+
 #include "norm_common.cuh"
 
 namespace pccl {
@@ -24,7 +26,7 @@ template <typename TX, typename TR, bool kFull> struct BackwardSlots {
   static constexpr int kGamma = 0, kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
   static constexpr int kDy = kBytes<TR>, kH = kDy + kBytes<TX>, kX = kH + kBytes<TR>;
   static constexpr int kShare = kX + (kReadsX ? kBytes<TX> : 0);
-  static int window(int threads) { return 2 * window_bytes<TR>(threads) + (kReadsX ? 2 : 1) * window_bytes<TX>(threads); }
+  static constexpr int kWindows = kReadsX ? 4 : 3;
 };
 
 template <typename T, bool kVec, int G>
@@ -34,21 +36,22 @@ __device__ __forceinline__ void store_weight_grad(void* out, int f32, int64_t fi
   else store_row<T, kVec, G>(static_cast<T*>(out) + first, c, f);
 }
 
-template <typename TX, typename TR, int kMode, bool kFull, int kMost>
-__global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParams p) {
+template <typename TX, typename TR, int kMode, bool kFull, bool kSplit>
+__global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormParams p) {
   using Slots = BackwardSlots<TX, TR, kFull>;
-  constexpr bool kVec = aligned_mode(kMode);
+  constexpr bool kVec = kMode == kRing;
   constexpr int G = kGroup<TX, TR>, kGroups = kHeld / G;
   __shared__ RowSums sums;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];         // rows of the ring begin with a line: 154 us instead of 168
   const NormArgs& a = p.a;
   const NormGrads& g = p.g;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
   asm volatile("griddepcontrol.launch_dependents;");
-  const Columns<kVec, G> c(n);
-  row_sum_clear(sums);
-  const int64_t begin = run_start(a.rows, p.workers, blockIdx.x), end = run_start(a.rows, p.workers, blockIdx.x + 1);
+  const int rank = kSplit ? cluster_rank() : 0, worker = static_cast<int>(blockIdx.x) / (kSplit ? kSplitBlocks : 1);
+  const Columns<kVec, G> c(n, rank);
+  row_sum_clear<kSplit>(sums);
+  const int64_t begin = run_start(a.rows, p.workers, worker), end = run_start(a.rows, p.workers, worker + 1);
 
   char* const gammas = smem;
   char* const g1 = smem + Slots::kG1 * width;
@@ -76,18 +79,17 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
         }
         if (reads_x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, c);
       } else {
-        if (g.dh) fetch_window(to, dh_rows + row * g.lddh, n);
+        if (g.dh) fetch_window(to, dh_rows + row * g.lddh, c);
         if (g.dy) {
-          fetch_window(to + off_dy, dy_rows + row * g.lddy, n);
-          fetch_window(to + off_h, stream + row * lds, n);
+          fetch_window(to + off_dy, dy_rows + row * g.lddy, c);
+          fetch_window(to + off_h, stream + row * lds, c);
         }
-        if (reads_x) fetch_window(to + off_x, x_rows + row * a.ldx, n);
+        if (reads_x) fetch_window(to + off_x, x_rows + row * a.ldx, c);
       }
     }
     copies_commit();
   };
-  if constexpr (kMode == kRing || kMode == kWindow)
-    for (int s = 0; s < p.ring - 1; ++s) fetch(begin + s, s);
+  for (int s = 0; s < p.ring - 1; ++s) fetch(begin + s, s);
 
   float2 acc_gamma[kHeld / 2], acc_s[kFull ? kHeld / 2 : 1];
 #pragma unroll
@@ -122,10 +124,15 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
     if constexpr (kMode == kRing) {
       fetch(t + p.ring - 1, last);
       copies_wait(p.ring - 1);
-    } else if constexpr (kMode == kWindow) {
+    } else if (p.ring > 1) {
       copies_wait(p.ring - 2);
       __syncthreads();                             // everybody's copies of this row, and the last one's readers
       fetch(t + p.ring - 1, last);
+    } else {
+      __syncthreads();
+      fetch(t, 0);
+      copies_wait(0);
+      __syncthreads();
     }
     s = s + 1 == p.ring ? 0 : s + 1;
     const TX* const row_x = x_rows + t * a.ldx;
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
           dot = fma2(d[v * (G / 2) + j], h[j], dot);
         }
       }
-      const float pull = -r2 * inv_n * row_sum(dot.x + dot.y, sums, &turn);
+      const float pull = -r2 * inv_n * row_sum<kSplit>(dot.x + dot.y, sums, &turn);
 #pragma unroll
       for (int i = 0; i < kHeld / 2; ++i) d[i] = fma2(both(r2), d[i], mul2(both(pull), n2[i]));
     } else {
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
     }
     if (kFull && a.post_gamma.ptr) {
       // n1 = r1 * x once more
-      const float pull = -r1 * r1 * inv_n * row_sum(dot.x + dot.y, sums, &turn);
+      const float pull = -r1 * r1 * inv_n * row_sum<kSplit>(dot.x + dot.y, sums, &turn);
       if (g.dx) {
 #pragma unroll
         for (int v = 0; v < kGroups; ++v) {
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
             float2 w[kHeld / 2];
             if (p.part_post) {
               // Added up in this thread's own columns of the block's part: once a group, so not worth registers.
-              float* const part = p.part_post + static_cast<int64_t>(blockIdx.x) * n;
+              float* const part = p.part_post + static_cast<int64_t>(worker) * n;
               load_weight<TX, kVec, G>(a.gate, group * n, c, w);
 #pragma unroll
               for (int v = 0; v < kGroups; ++v) {
@@ -243,7 +250,7 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
               store_weight_grad<TX, kVec, G>(g.dgate, a.gate.f32, group * n, c, acc_s);
             } else {
               const int slot = group * a.gate_rows <= begin ? 0 : 1;
-              store_row<float, kVec, G>(p.part_gate + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * n, c, acc_s);
+              store_row<float, kVec, G>(p.part_gate + (static_cast<int64_t>(worker) * 2 + slot) * n, c, acc_s);
             }
           }
 #pragma unroll
@@ -254,11 +261,11 @@ __global__ void __launch_bounds__(kMost, 1) norm_backward_kernel(const NormParam
       }
     }
   }
-  if constexpr (kMode == kRing || kMode == kWindow) copies_wait(0);
-  if (p.part_gamma) store_row<float, kVec, G>(p.part_gamma + static_cast<int64_t>(blockIdx.x) * n, c, acc_gamma);
+  copies_wait(0);
+  if (p.part_gamma) store_row<float, kVec, G>(p.part_gamma + static_cast<int64_t>(worker) * n, c, acc_gamma);
   if constexpr (kFull) {
     if (p.part_post && !a.gate.ptr) {
-      store_row<float, kVec, G>(p.part_post + static_cast<int64_t>(blockIdx.x) * n, c, acc_s);
+      store_row<float, kVec, G>(p.part_post + static_cast<int64_t>(worker) * n, c, acc_s);
     }
   }
 }
@@ -342,63 +349,75 @@ template <typename T, int C> void reduce_launch(const NormParams& p, cudaStream_
   PCCL_CUDA(cudaLaunchKernelEx(&config, norm_reduce_kernel<T, C>, p));
 }
 
-// Blocks of the backward kernel: what an SM holds of them, each with at least one row.
-int worker_count(const NormArgs& a) {
-  const int per_sm = blocks_per_sm(threads_of(a.hidden));
-  const int64_t most = static_cast<int64_t>(per_sm) * sm_count();
-  return static_cast<int>(a.rows < most ? a.rows : most);
-}
-
-template <typename TX, typename TR, bool kFull, int kMost>
-void backward_mode(NormParams& p, bool vec, int threads, cudaStream_t stream) {
+// How rows are laid out, and how many clusters share them: what the SMs hold, each with at least one row.
+template <typename TX, typename TR, bool kFull> Layout backward_layout(const NormArgs& a, bool vec, int* workers) {
   using Slots = BackwardSlots<TX, TR, kFull>;
-  const RingSize size{threads, Slots::kWeights, Slots::kShare, Slots::window(threads)};
-  size_t smem = 0;
-  switch (choose_mode(size, vec, &p.ring, &smem)) {
-    case kRing: launch(norm_backward_kernel<TX, TR, kRing, kFull, kMost>, p, threads, smem, stream); break;
-    case kWindow: launch(norm_backward_kernel<TX, TR, kWindow, kFull, kMost>, p, threads, smem, stream); break;
-    case kDirect: launch(norm_backward_kernel<TX, TR, kDirect, kFull, kMost>, p, threads, smem, stream); break;
-    default: launch(norm_backward_kernel<TX, TR, kScalar, kFull, kMost>, p, threads, smem, stream); break;
-  }
+  const Layout l = layout_of(a.hidden, vec, Slots::kWeights, Slots::kShare, Slots::kWindows, 512, false);
+  const int64_t most = static_cast<int64_t>(blocks_per_sm(l.threads)) * sm_count() / l.split;
+  *workers = static_cast<int>(a.rows < most ? a.rows : most);
+  return l;
 }
 
-template <typename TX, typename TR>
-void backward_typed(NormParams& p, bool vec, cudaStream_t stream) {
-  const int threads = threads_of(p.a.hidden);
-  const bool full = has_g1(p.a);
-  if (threads > 512 && full) backward_mode<TX, TR, true, 1024>(p, vec, threads, stream);
-  else if (threads > 512) backward_mode<TX, TR, false, 1024>(p, vec, threads, stream);
-  else if (full) backward_mode<TX, TR, true, 512>(p, vec, threads, stream);
-  else backward_mode<TX, TR, false, 512>(p, vec, threads, stream);
+template <typename TX, typename TR, bool kFull>
+void backward_mode(NormParams& p, bool vec, cudaStream_t stream) {
+  const Layout l = backward_layout<TX, TR, kFull>(p.a, vec, &p.workers);
+  p.ring = l.ring;
+  if (vec && l.split > 1) launch(norm_backward_kernel<TX, TR, kRing, kFull, true>, p, l, stream);
+  else if (vec) launch(norm_backward_kernel<TX, TR, kRing, kFull, false>, p, l, stream);
+  else if (l.split > 1) launch(norm_backward_kernel<TX, TR, kWindow, kFull, true>, p, l, stream);
+  else launch(norm_backward_kernel<TX, TR, kWindow, kFull, false>, p, l, stream);
+}
+
+// Calls f.template operator()<TX, TR, kFull>() for the types and weights of these arguments.
+template <class F> void with_types(const NormArgs& a, F f) {
+  PCCL_BLOCK_TYPES(a.xt, T,
+    if (a.rt == a.xt && has_g1(a)) f(T(), T(), std::true_type());
+    else if (a.rt == a.xt) f(T(), T(), std::false_type());
+    else if (has_g1(a)) f(T(), float(), std::true_type());
+    else f(T(), float(), std::false_type()))
+}
+
+bool all_aligned(const NormArgs& a, const NormGrads& g) {
+  const int xb = dtype_bytes(a.xt), rb = dtype_bytes(a.rt);
+  return inputs_aligned(a) && aligned(g.dy, g.lddy, xb) && aligned(g.dh, g.lddh, rb) && aligned(g.h, a.hidden, 4) &&
+         aligned(g.dx, a.hidden, xb) && aligned(g.dresidual, a.hidden, rb) &&
+         aligned(g.dgate, a.hidden, a.gate.f32 ? 4 : xb) && aligned(g.workspace, a.hidden, 4);
 }
 
 }  // namespace
 }  // namespace norm
 
 size_t norm_workspace(const NormArgs& a, const NormGrads& g) {
-  const size_t row = static_cast<size_t>(norm::worker_count(a)) * a.hidden * sizeof(float);
+  // Either way of reading rows may be taken: the larger count of workers.
+  int most = 0;
+  norm::with_types(a, [&](auto x, auto r, auto full) {
+    for (const bool vec : {true, false}) {
+      int workers = 0;
+      norm::backward_layout<decltype(x), decltype(r), decltype(full)::value>(a, vec, &workers);
+      most = workers > most ? workers : most;
+    }
+  });
+  const size_t row = static_cast<size_t>(most) * a.hidden * sizeof(float);
   return row * ((g.dgamma ? 1 : 0) + (g.dpost_gamma ? 1 : 0) + (g.dgate ? 2 : 0));
 }
 
 void norm_backward(const NormArgs& a, const NormGrads& g, cudaStream_t stream) {
   if (a.rows == 0) return;
-  using norm::aligned;
   norm::NormParams p{};
   p.a = a;
   p.g = g;
-  p.workers = norm::worker_count(a);
+  const bool vec = norm::all_aligned(a, g);
+  norm::with_types(a, [&](auto x, auto r, auto full) {
+    norm::backward_layout<decltype(x), decltype(r), decltype(full)::value>(a, vec, &p.workers);
+  });
   const int64_t row = static_cast<int64_t>(p.workers) * a.hidden;
   float* at = static_cast<float*>(g.workspace);
   if (g.dgamma) { p.part_gamma = at; at += row; }
   if (g.dpost_gamma) { p.part_post = at; at += row; }
   if (g.dgate) p.part_gate = at;
-  const int xb = dtype_bytes(a.xt), rb = dtype_bytes(a.rt);
-  const bool vec = norm::inputs_aligned(a) && aligned(g.dy, g.lddy, xb) && aligned(g.dh, g.lddh, rb) &&
-                   aligned(g.h, a.hidden, 4) && aligned(g.dx, a.hidden, xb) && aligned(g.dresidual, a.hidden, rb) &&
-                   aligned(g.dgate, a.hidden, a.gate.f32 ? 4 : xb) && aligned(g.workspace, a.hidden, 4);
-  PCCL_BLOCK_TYPES(a.xt, T,
-    if (a.rt == a.xt) norm::backward_typed<T, T>(p, vec, stream);
-    else norm::backward_typed<T, float>(p, vec, stream))
+  norm::with_types(a, [&](auto x, auto r, auto full) {
+    norm::backward_mode<decltype(x), decltype(r), decltype(full)::value>(p, vec, stream);
+  });
   PCCL_CUDA(cudaGetLastError());
   if (g.dgamma || g.dpost_gamma || g.dgate) {
     PCCL_BLOCK_TYPES(a.xt, T,

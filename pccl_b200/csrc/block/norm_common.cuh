@@ -2,13 +2,17 @@
 //
 // Both kernels are bound by memory, and what keeps memory waiting is a row's own chain: load, sum over the row,
 // barrier, use, perhaps a second sum.  So the coming rows are on their way into a ring in shared memory (cp.async,
-// which holds no registers) while a block works on the present one.  Four ways of reading a row:
+// which holds no registers) while a block works on the present one.  Two ways of reading a row:
 //
 //   kRing     rows aligned to 16 bytes: every thread copies the columns it will use into slots of its own, so no
 //             barrier is needed to read them;
 //   kWindow   rows that begin anywhere (odd sizes, cut views): the block copies the 16-byte blocks that cover the
-//             row and picks the values out of shared memory;
-//   kDirect, kScalar   rows too long for the ring, loaded where they are used, by 16 bytes or one by one.
+//             row and picks the values out of shared memory.
+//
+// Rows too long for one block's registers or ring are split over a cluster of two blocks, which add up their sums
+// through one another's shared memory: 12288 columns of bf16 backwards with all weights run at 2.5 TB/s so, at 1.9 in
+// one block of 1024 threads, whose 64 registers each spill; over four blocks at 1.6, since a barrier of a cluster is
+// most of a microsecond.  Forwards 64 registers suffice, and one block comes first (5.3 TB/s against 3.5).
 #pragma once
 #include "../common/launch.h"
 #include "../common/util.h"
@@ -20,8 +24,8 @@ namespace block {
 namespace norm {
 
 constexpr int kHeld = 16;                      // values a thread holds of its row
-enum Mode : int { kRing = 0, kWindow = 1, kDirect = 2, kScalar = 3 };
-constexpr bool aligned_mode(int m) { return m == kRing || m == kDirect; }
+enum Mode : int { kRing = 0, kWindow = 1 };
+constexpr int kSplitBlocks = 2;                // of a cluster that shares a row
 
 // A thread's values stand in groups of consecutive columns, as many as 16 bytes of the widest type hold: a warp then
 // touches whole 32-byte sectors in every access.  (Eight columns of 32 bits a thread, as two accesses 32 bytes apart
@@ -38,7 +42,7 @@ struct NormParams {
   float* part_gamma;          // [workers][hidden]
   float* part_post;           // [workers][hidden]
   float* part_gate;           // [workers][2][hidden]: the run's first group of rows, its last one
-  int workers;                // blocks, each with a run of consecutive rows
+  int workers;                // blocks, or clusters of them, each with a run of consecutive rows
   int ring;                   // rows in shared memory
 };
 
@@ -46,10 +50,15 @@ struct NormParams {
 // else one of every 32.  Steps from one access to the next are constants then, which matters: with a step of the
 // block's width a third of all instructions were addresses.
 template <bool kVec, int G> struct Columns {
-  int first;                  // this thread's first column
-  int room;                   // columns from there to the row's end
-  __device__ explicit Columns(int hidden) {
-    first = static_cast<int>(threadIdx.x >> 5) * 32 * kHeld + static_cast<int>(threadIdx.x & 31) * (kVec ? G : 1);
+  int part, columns;          // the block's first column, and how many it has
+  int local;                  // this thread's first column within the block's
+  int first, room;            // the same within the row, and the columns from there to the row's end
+  __device__ Columns(int hidden, int rank) {
+    const int held = static_cast<int>(blockDim.x) * kHeld;
+    part = rank * held;
+    columns = max(min(hidden - part, held), 0);
+    local = static_cast<int>(threadIdx.x >> 5) * 32 * kHeld + static_cast<int>(threadIdx.x & 31) * (kVec ? G : 1);
+    first = part + local;
     room = hidden - first;
   }
 };
@@ -149,20 +158,20 @@ __device__ __forceinline__ void fetch_share(char* image, const T* row, const Col
 #pragma unroll
   for (int v = 0; v < kHeld / G; ++v) {
     const bool beyond = v * 32 * G >= c.room;
-    copy_async<kSize>(image + c.first * static_cast<int>(sizeof(T)) + v * 32 * kSize, beyond ? row : row + c.first + v * 32 * G,
+    copy_async<kSize>(image + c.local * static_cast<int>(sizeof(T)) + v * 32 * kSize, beyond ? row : row + c.first + v * 32 * G,
                       beyond ? 0 : kSize);
   }
 }
 
 // Bytes of a window for any row of T.
 template <typename T> __host__ __device__ constexpr int window_bytes(int threads) { return threads * kBytes<T> + 16; }
-// The 16-byte blocks that cover the row, and zeros up to the last column that a thread holds.  The first may begin with
-// values in front of the row: such a block holds a value of the row, and allocations begin at multiples of 256
+// The 16-byte blocks that cover the block's part of the row, and zeros up to the last column that a thread holds.  The first may begin with
+// values in front of it: such a block holds a value of the row, and allocations begin at multiples of 256
 // bytes, so all of it is theirs.  Nothing is read behind the row.
-template <typename T>
-__device__ __forceinline__ void fetch_window(char* window, const T* row, int hidden) {
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(row);
-  const int ahead = static_cast<int>(begin & 15), bytes = ahead + hidden * static_cast<int>(sizeof(T));
+template <typename T, int G>
+__device__ __forceinline__ void fetch_window(char* window, const T* row, const Columns<false, G>& c) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(row + c.part);
+  const int ahead = static_cast<int>(begin & 15), bytes = ahead + c.columns * static_cast<int>(sizeof(T));
   const char* const first = reinterpret_cast<const char*>(begin - ahead);
   const int all = window_bytes<T>(static_cast<int>(blockDim.x));
   for (int at = static_cast<int>(threadIdx.x) * 16; at < all; at += static_cast<int>(blockDim.x) * 16) {
@@ -173,38 +182,62 @@ __device__ __forceinline__ void fetch_window(char* window, const T* row, int hid
 
 // Group v of a row of T; `held` is the row's image in the ring, or its window.
 template <typename T, int kMode, int G>
-__device__ __forceinline__ void take(const char* held, const T* row, int v, const Columns<aligned_mode(kMode), G>& c, float2* to) {
+__device__ __forceinline__ void take(const char* held, const T* row, int v, const Columns<kMode == kRing, G>& c, float2* to) {
   if constexpr (kMode == kRing) {
-    unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(held + c.first * static_cast<int>(sizeof(T)) + v * static_cast<int>(32 * G * sizeof(T))), to);
-  } else if constexpr (kMode == kWindow) {
-    const T* at = reinterpret_cast<const T*>(held + (reinterpret_cast<uintptr_t>(row) & 15)) + c.first;
+    unpack<T, G>(*reinterpret_cast<const Raw<T, G>*>(held + c.local * static_cast<int>(sizeof(T)) + v * static_cast<int>(32 * G * sizeof(T))), to);
+  } else {
+    const T* at = reinterpret_cast<const T*>(held + (reinterpret_cast<uintptr_t>(row + c.part) & 15)) + c.local;
     float* f = reinterpret_cast<float*>(to);
 #pragma unroll
     for (int j = 0; j < G; ++j) f[j] = to_f32<T>(at[(v * G + j) * 32]);
-  } else {
-    load_group<T, kMode == kDirect, G>(row, v, c, to);
   }
 }
 
-// Sum over the block; `sums` alternates between two sets so that one barrier a call is enough.  Sets are cleared
-// once (row_sum_clear), so that whole groups of four can be read.
-struct __align__(16) RowSums { float set[2][32]; };
-__device__ __forceinline__ void row_sum_clear(RowSums& sums) {
+// Sum over a row; `sums` alternates between two sets so that one barrier a call is enough.  Sets are cleared once
+// (row_sum_clear), so that whole groups of four can be read.  Blocks that share a row send one another their sums
+// and add them in the order of their ranks, so all get the same.
+struct __align__(16) RowSums {
+  float set[2][32];
+  float block[2][kSplitBlocks];
+};
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <bool kSplit> __device__ __forceinline__ void row_sum_clear(RowSums& sums) {
   if (blockDim.x == 32) return;
   if (threadIdx.x < 64) (&sums.set[0][0])[threadIdx.x] = 0.f;
-  __syncthreads();
+  if constexpr (kSplit) cluster_barrier();         // every block has begun before one writes to it
+  else __syncthreads();
 }
-__device__ __forceinline__ float row_sum(float v, RowSums& sums, int* turn) {
+template <bool kSplit> __device__ __forceinline__ float row_sum(float v, RowSums& sums, int* turn) {
   v = warp_sum(v);
-  if (blockDim.x == 32) return v;
-  float* s = sums.set[*turn];
+  if (blockDim.x == 32) return v;                  // a split row has more threads
+  const int now = *turn;
   *turn ^= 1;
+  float* s = sums.set[now];
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0.f;
   for (int w = 0; w < static_cast<int>(blockDim.x >> 5); w += 4) {
     const float4 q = *reinterpret_cast<const float4*>(s + w);
     v += (q.x + q.y) + (q.z + q.w);
+  }
+  if constexpr (kSplit) {
+    if (threadIdx.x < kSplitBlocks) {
+      const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&sums.block[now][cluster_rank()]));
+      uint32_t theirs;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(static_cast<int>(threadIdx.x)));
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(theirs), "f"(v) : "memory");
+    }
+    cluster_barrier();
+    v = 0.f;
+#pragma unroll
+    for (int r = 0; r < kSplitBlocks; ++r) v += sums.block[now][r];
   }
   return v;
 }
@@ -245,7 +278,7 @@ __device__ __forceinline__ int64_t run_start(int64_t rows, int workers, int w) {
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
-inline int threads_of(int hidden) { return ((hidden + kHeld - 1) / kHeld + 31) / 32 * 32; }
+inline int threads_of(int hidden, int split) { return ((hidden + split * kHeld - 1) / (split * kHeld) + 31) / 32 * 32; }
 
 inline int sm_count() {
   int dev = 0, sms = 0;
@@ -270,38 +303,55 @@ inline bool inputs_aligned(const NormArgs& a) {
 constexpr size_t kSmemSm = 228 * 1024, kSmemBlock = 226 * 1024, kSmemKept = 1024 + sizeof(RowSums);
 constexpr int kMostRing = 4;
 
-// Shared memory of a block with `rows` rows in the ring.
-struct RingSize {
-  int threads;
-  int weights, share;         // bytes a thread: weights, its share of one row (kRing)
-  int window;                 // bytes of one row's windows
-  size_t bytes(int mode, int rows) const {
-    return static_cast<size_t>(weights + (mode == kRing ? rows * share : 0)) * threads +
-           (mode == kWindow ? static_cast<size_t>(rows) * window : 0);
-  }
-  // As many rows as leave `blocks` blocks on an SM, at least two; 0 where two do not fit into one.
-  int rows(int mode, int blocks) const {
-    for (int r = kMostRing; r > 2; --r)
-      if ((bytes(mode, r) + kSmemKept) * blocks <= kSmemSm && bytes(mode, r) <= kSmemBlock) return r;
-    return bytes(mode, 2) <= kSmemBlock ? 2 : 0;
-  }
+// How a row of `hidden` columns is laid out over blocks.  weights and share are bytes a thread, of its weights and of
+// its share of a row; windows is how many windows a row has beyond those bytes.
+struct Layout {
+  int mode, split, threads, ring;
+  size_t smem;
 };
 // Registers let 512 threads of 128 registers (or 1024 of 64) share an SM.
 inline int blocks_per_sm(int threads) { return threads < 512 ? 512 / threads : 1; }
 
-// The mode for these rows; *ring and *smem go with it.
-inline int choose_mode(const RingSize& size, bool vec, int* ring, size_t* smem) {
-  int mode = vec ? kRing : kWindow;
-  *ring = size.rows(mode, blocks_per_sm(size.threads));
-  if (*ring == 0) mode = vec ? kDirect : kScalar;
-  *smem = size.bytes(mode, *ring);
-  return mode;
+// Tries blocks of up to `most_threads`, and where these are too few or leave no room for the ring, clusters of two;
+// `alone`: a block without room for a row on its way comes before a cluster.
+inline Layout layout_of(int hidden, bool vec, int weights, int share, int windows, int most_threads, bool alone) {
+  Layout l{};
+  const auto fits = [&](int split, int least) {
+    l = Layout{vec ? kRing : kWindow, split, threads_of(hidden, split), 0, 0};
+    if (l.threads > most_threads) return false;
+    const auto bytes = [&](int rows) {
+      return static_cast<size_t>(weights + rows * share) * l.threads + (vec ? 0 : static_cast<size_t>(rows) * windows * 16);
+    };
+    // As many rows as leave room for the blocks that registers have room for.
+    for (int r = kMostRing; r >= least && l.ring == 0; --r)
+      if (bytes(r) <= kSmemBlock && (r <= 2 || (bytes(r) + kSmemKept) * blocks_per_sm(l.threads) <= kSmemSm)) l.ring = r;
+    l.smem = bytes(l.ring);
+    return l.ring > 0;
+  };
+  const bool found = fits(1, 2) || (alone && fits(1, 1)) || fits(kSplitBlocks, 2) || fits(kSplitBlocks, 1);
+  PCCL_CHECK(found, "block norm: a row of " << hidden << " columns does not fit");
+  return l;
 }
 
-template <class Kernel> void launch(Kernel kernel, const NormParams& p, int threads, size_t smem, cudaStream_t stream) {
-  if (smem > 40 * 1024)
-    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  kernel<<<p.workers, threads, smem, stream>>>(p);
+template <class Kernel> void launch(Kernel kernel, const NormParams& p, const Layout& l, cudaStream_t stream) {
+  if (l.smem > 40 * 1024)
+    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.smem)));
+  if (l.split == 1) {
+    kernel<<<p.workers, l.threads, l.smem, stream>>>(p);
+    return;
+  }
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = l.split;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(p.workers * l.split);
+  config.blockDim = dim3(l.threads);
+  config.dynamicSmemBytes = l.smem;
+  config.stream = stream;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  PCCL_CUDA(cudaLaunchKernelEx(&config, kernel, p));
 }
 
 }  // namespace norm

@@ -6,6 +6,8 @@
 //
 // y is formed from h as it stands in 32 bits, before its rounding to the stream's type.  post_gamma and gate wait in
 // shared memory as their product g1.
+#include <type_traits>
+
 #include "norm_common.cuh"
 
 namespace pccl {
@@ -19,19 +21,20 @@ template <typename TX, typename TR, bool kFull> struct ForwardSlots {
   static constexpr int kX = kBytes<TR>, kShare = kBytes<TR> + kBytes<TX>;
 };
 
-template <typename TX, typename TR, int kMode, bool kFull, int kMost>
+template <typename TX, typename TR, int kMode, bool kFull, bool kSplit, int kMost>
 __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams p) {
   using Slots = ForwardSlots<TX, TR, kFull>;
-  constexpr bool kVec = aligned_mode(kMode);
+  constexpr bool kVec = kMode == kRing;
   constexpr int G = kGroup<TX, TR>, kGroups = kHeld / G;
   __shared__ RowSums sums;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];
   const NormArgs& a = p.a;
   const int tid = threadIdx.x, width = blockDim.x, n = a.hidden;
   const float inv_n = 1.f / static_cast<float>(n);
-  const Columns<kVec, G> c(n);
-  row_sum_clear(sums);
-  const int64_t begin = run_start(a.rows, p.workers, blockIdx.x), end = run_start(a.rows, p.workers, blockIdx.x + 1);
+  const int rank = kSplit ? cluster_rank() : 0, worker = static_cast<int>(blockIdx.x) / (kSplit ? kSplitBlocks : 1);
+  const Columns<kVec, G> c(n, rank);
+  row_sum_clear<kSplit>(sums);
+  const int64_t begin = run_start(a.rows, p.workers, worker), end = run_start(a.rows, p.workers, worker + 1);
 
   char* const gammas = smem;
   char* const g1 = smem + Slots::kG1 * width;
@@ -47,14 +50,13 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
         fetch_share<TR, G>(to, residual + row * a.ldr, c);
         if (a.x) fetch_share<TX, G>(to + off_x, x_rows + row * a.ldx, c);
       } else {
-        fetch_window(to, residual + row * a.ldr, n);
-        if (a.x) fetch_window(to + off_x, x_rows + row * a.ldx, n);
+        fetch_window(to, residual + row * a.ldr, c);
+        if (a.x) fetch_window(to + off_x, x_rows + row * a.ldx, c);
       }
     }
     copies_commit();
   };
-  if constexpr (kMode == kRing || kMode == kWindow)
-    for (int s = 0; s < p.ring - 1; ++s) fetch(begin + s, s);
+  for (int s = 0; s < p.ring - 1; ++s) fetch(begin + s, s);
 
   if (a.gamma.ptr) {
     float2 w[kHeld / 2];
@@ -75,10 +77,15 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
     if constexpr (kMode == kRing) {
       fetch(t + p.ring - 1, last);
       copies_wait(p.ring - 1);
-    } else if constexpr (kMode == kWindow) {
+    } else if (p.ring > 1) {
       copies_wait(p.ring - 2);
       __syncthreads();                             // everybody's copies of this row, and the last one's readers
       fetch(t + p.ring - 1, last);
+    } else {
+      __syncthreads();
+      fetch(t, 0);
+      copies_wait(0);
+      __syncthreads();
     }
     s = s + 1 == p.ring ? 0 : s + 1;
     float2 x[kHeld / 2], h[kHeld / 2];
@@ -94,8 +101,8 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
       }
       if constexpr (kFull) {
         if (a.post_gamma.ptr) {
-          r1 = rsqrtf(row_sum(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
-          if (p.r1 && tid == 0) p.r1[t] = r1;
+          r1 = rsqrtf(row_sum<kSplit>(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
+          if (p.r1 && tid == 0 && rank == 0) p.r1[t] = r1;
         }
         if (left == 0) {
           form_g1<TX, kVec, G>(a, ++group, g1, c);
@@ -124,8 +131,8 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
       if (p.h) store_group<TR, kVec, G>(static_cast<TR*>(p.h) + t * n, v, c, hv);
     }
     if (a.gamma.ptr) {
-      const float r2 = rsqrtf(row_sum(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
-      if (p.r2 && tid == 0) p.r2[t] = r2;
+      const float r2 = rsqrtf(row_sum<kSplit>(ss.x + ss.y, sums, &turn) * inv_n + a.eps);
+      if (p.r2 && tid == 0 && rank == 0) p.r2[t] = r2;
 #pragma unroll
       for (int v = 0; v < kGroups; ++v) {
         float2 w[G / 2];
@@ -136,42 +143,41 @@ __global__ void __launch_bounds__(kMost, 1) norm_forward_kernel(const NormParams
       }
     }
   }
-  if constexpr (kMode == kRing || kMode == kWindow) copies_wait(0);
+  copies_wait(0);
 }
 
-template <typename TX, typename TR, int kMode, bool kFull, int kMost>
-void forward_launch(NormParams& p, int threads, size_t smem, cudaStream_t stream) {
+template <typename TX, typename TR, int kMode, bool kFull, bool kSplit, int kMost>
+void forward_launch(NormParams& p, const Layout& l, cudaStream_t stream) {
   // One wave of blocks: a block's later rows are on their way while it works.
-  const auto kernel = norm_forward_kernel<TX, TR, kMode, kFull, kMost>;
-  if (smem > 40 * 1024)
-    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  const int64_t most = max_coresident(kernel, threads, smem);
+  const auto kernel = norm_forward_kernel<TX, TR, kMode, kFull, kSplit, kMost>;
+  if (l.smem > 40 * 1024)
+    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.smem)));
+  const int64_t most = static_cast<int64_t>(max_coresident(kernel, l.threads, l.smem)) / l.split;
   PCCL_CHECK(most > 0, "block norm: the kernel does not fit on this device");
   p.workers = static_cast<int>(p.a.rows < most ? p.a.rows : most);
-  launch(kernel, p, threads, smem, stream);
+  p.ring = l.ring;
+  launch(kernel, p, l, stream);
 }
 
-template <typename TX, typename TR, bool kFull, int kMost>
-void forward_mode(NormParams& p, bool vec, int threads, cudaStream_t stream) {
+template <typename TX, typename TR, bool kFull>
+void forward_mode(NormParams& p, bool vec, cudaStream_t stream) {
   using Slots = ForwardSlots<TX, TR, kFull>;
-  const RingSize size{threads, Slots::kWeights, Slots::kShare, window_bytes<TR>(threads) + window_bytes<TX>(threads)};
-  size_t smem = 0;
-  switch (choose_mode(size, vec, &p.ring, &smem)) {
-    case kRing: forward_launch<TX, TR, kRing, kFull, kMost>(p, threads, smem, stream); break;
-    case kWindow: forward_launch<TX, TR, kWindow, kFull, kMost>(p, threads, smem, stream); break;
-    case kDirect: forward_launch<TX, TR, kDirect, kFull, kMost>(p, threads, smem, stream); break;
-    default: forward_launch<TX, TR, kScalar, kFull, kMost>(p, threads, smem, stream); break;
-  }
+  // One block a row as long as it fits (12288 columns of bf16: 5.3 TB/s so, 3.5 split over two).
+  const Layout l = layout_of(p.a.hidden, vec, Slots::kWeights, Slots::kShare, 2, 1024, true);
+  const auto go = [&](auto mode) {
+    constexpr int kMode = decltype(mode)::value;
+    if (l.split > 1) forward_launch<TX, TR, kMode, kFull, true, 512>(p, l, stream);
+    else if (l.threads > 512) forward_launch<TX, TR, kMode, kFull, false, 1024>(p, l, stream);
+    else forward_launch<TX, TR, kMode, kFull, false, 512>(p, l, stream);
+  };
+  if (vec) go(std::integral_constant<int, kRing>());
+  else go(std::integral_constant<int, kWindow>());
 }
 
 template <typename TX, typename TR>
 void forward_typed(NormParams& p, bool vec, cudaStream_t stream) {
-  const int threads = threads_of(p.a.hidden);
-  const bool full = has_g1(p.a);
-  if (threads > 512 && full) forward_mode<TX, TR, true, 1024>(p, vec, threads, stream);
-  else if (threads > 512) forward_mode<TX, TR, false, 1024>(p, vec, threads, stream);
-  else if (full) forward_mode<TX, TR, true, 512>(p, vec, threads, stream);
-  else forward_mode<TX, TR, false, 512>(p, vec, threads, stream);
+  if (has_g1(p.a)) forward_mode<TX, TR, true>(p, vec, stream);
+  else forward_mode<TX, TR, false>(p, vec, stream);
 }
 
 }  // namespace
