@@ -88,6 +88,12 @@ ROUTES = [
     (5000, 40, 4, dict(bias=True)),
     (20000, 32, 3, dict(groups=32, top_groups=5)),
     (64, 2, 1, dict(groups=2, top_groups=1)),
+    # Around the sizes at which tokens go to more blocks, and lanes to more experts.
+    (24, 9, 3, dict()), (25, 9, 3, dict(bias=True)), (148 * 8 + 1, 65, 9, dict()), (148 * 32 + 3, 33, 2, dict(scoring="sigmoid")),
+    (1024, 8, 2, dict(bias=True)), (1025, 5, 5, dict(groups=5, top_groups=5)), (129, 31, 31, dict(renormalise=False)),
+    (200, 192, 7, dict(groups=4, top_groups=3, bias=True)), (150, 192, 7, dict(groups=6, top_groups=3, group_score="top2")),
+    (99, 510, 12, dict(groups=3, top_groups=2, bias=True, scoring="sigmoid")),
+    (180, 8, 3, dict(groups=4, top_groups=2, group_score="top2", scoring="sigmoid", bias=True)),
 ]
 
 
@@ -128,6 +134,29 @@ def test_route_tells_near_scores_apart(scoring):
     assert got.idx.unique().numel() == 8                          # the same choice for the same row
     _check_route(logits + 1e-6 * _normal(g, 600, 64), 8, bias=bias, scoring=scoring)
     _check_route(logits + 1e-6 * _normal(g, 600, 64), 8, bias=bias, scoring=scoring, groups=8, top_groups=3, group_score="top2")
+
+
+@pytest.mark.parametrize("experts", [8, 40, 256])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_ranks_near_pairs_again(scoring, experts):
+    """Pairs of scores a few units of the last place apart, at every place of the choice and just behind it."""
+    g = _gen(14)
+    tokens, k = 400, min(6, experts // 2)
+    logits = _normal(g, 1, experts).repeat(tokens, 1)
+    p = ref.probabilities(logits[:1].double(), scoring)[0]
+    bias = 0.05 * _normal(g, experts)
+    ranked = ref.order((p + bias.double())[None])[0]
+    for i in range(0, k + 1, 2):                                      # choice i + 1 meets choice i, the last the runner-up
+        a, b = ranked[i], ranked[i + 1]
+        bias[b] = (p[a] + bias[a].double() - p[b]).float()
+    logits += 2e-7 * _normal(g, tokens, experts)
+    _check_route(logits, k, bias=bias, scoring=scoring)
+    _check_route(logits, k, bias=bias, scoring=scoring, groups=4, top_groups=2, group_score="top2")
+    near = _normal(g, tokens, experts)                               # and logits alone, some equal, some a unit apart
+    near[:, 1::2] = near[:, ::2]
+    near[::3, 1::2] = torch.nextafter(near[::3, ::2], torch.full((), 10.0, device="cuda"))
+    _check_route(near, k, scoring=scoring)
+    _check_route(near, k, scoring=scoring, groups=4, top_groups=2)
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
@@ -262,7 +291,8 @@ def _check_moves(x, y, routing):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tokens,hidden,experts,top_k,live", [
     (1, 1, 1, 1, 1.0), (1, 4096, 8, 2, 1.0), (7, 33, 8, 3, 1.0), (300, 512, 16, 8, 1.0), (333, 1431, 60, 5, 0.8),
-    (50, 7, 8, 8, 0.5), (1025, 2056, 8, 2, 0.9), (64, 8200, 128, 31, 1.0), (3, 20001, 4, 1, 1.0), (200, 100, 9, 9, 0.0)])
+    (50, 7, 8, 8, 0.5), (1025, 2056, 8, 2, 0.9), (64, 8200, 128, 31, 1.0), (3, 20001, 4, 1, 1.0), (200, 100, 9, 9, 0.0), (5000, 8, 8, 2, 0.9), (3001, 64, 16, 6, 1.0), (2500, 200, 8, 3, 0.9),
+    (700, 1, 4, 4, 1.0)])
 def test_dispatch_and_combine(tokens, hidden, experts, top_k, live, dtype):
     g = _gen(tokens + hidden)
     routing = _routing(g, tokens, experts, top_k, live, requires_grad=True)
@@ -394,7 +424,8 @@ NORMS = [
     ((999,), 513, True, True, 1, 1.0), ((700,), 1000, False, True, 7, 2.0), ((602,), 2055, True, True, 2, 1.0),
     ((301,), 4096, False, False, 1, 1.0), ((6, 100), 2048, True, True, 6, 0.9), ((64,), 8192, True, True, 64, 1.0),
     ((37,), 16384, True, True, 1, 1.0), ((9,), 16383, True, True, 3, 1.0), ((2000,), 256, False, False, 0, 0.7),
-    ((5000,), 136, True, True, 4, 1.0),
+    ((5000,), 136, True, True, 4, 1.0), ((400,), 8200, True, True, 4, 1.0), ((333,), 12289, True, True, 9, 0.9),
+    ((500,), 10240, True, False, 0, 1.0), ((211,), 16384, True, True, 211, 1.0), ((300,), 9001, False, True, 0, 1.0),
 ]
 
 
@@ -429,6 +460,21 @@ def test_norm_gradients_of_one_output_and_32_bit_weights(use, post, rt):
 def test_rms_norm(rows, hidden, dtype):
     g = _gen(rows)
     _check_norm(_normal(g, rows, hidden).to(dtype), None, (1 + 0.1 * _normal(g, hidden)).to(dtype), None, None)
+
+
+def test_norm_of_one_tensor_twice():
+    g = _gen(18)
+    x = _normal(g, 70, 320).bfloat16().requires_grad_(True)
+    gamma = (1 + 0.1 * _normal(g, 320)).bfloat16()
+    y, h = residual_rms_norm(x, x, gamma)
+    dy, dh = _normal(g, 70, 320).bfloat16(), _normal(g, 70, 320).bfloat16()
+    both, = torch.autograd.grad((y, h), x, (dy, dh))
+    a, b = x.detach().clone().requires_grad_(True), x.detach().clone().requires_grad_(True)
+    parts = torch.autograd.grad(residual_rms_norm(a, b, gamma), (a, b), (dy, dh))
+    assert torch.equal(both, parts[0] + parts[1])
+    y, h = residual_rms_norm(x, x, gamma)
+    (y.float().sum() + h.float().sum()).backward()
+    assert x.grad.shape == x.shape
 
 
 def test_norm_of_zero_rows_and_rows_of_zeros():
@@ -526,6 +572,34 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(want[i], got[i]))
+
+
+def test_long_rows_captured():
+    """Rows that two blocks share, forward and backward, captured and replayed on other inputs."""
+    def make(seed):
+        g = _gen(seed)
+        return [t.requires_grad_(True) for t in (_normal(g, 300, 9216).bfloat16(), _normal(g, 300, 9216).bfloat16(),
+                                                 (1 + 0.1 * _normal(g, 9216)).bfloat16(), _normal(g, 3, 9216).bfloat16())]
+
+    def step(stream, x, gamma, gate):
+        y, h = residual_rms_norm(stream, x, gamma, post_gamma=gamma, gate=gate)
+        return torch.autograd.grad(y.float().square().sum() + h.float().sum(), (stream, x, gamma, gate))
+
+    args = make(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*args)
+    fresh = make(2)
+    for a, b in zip(args, fresh):
+        a.data.copy_(b.data)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, step(*fresh)))
 
 
 def test_two_captured_graphs():
