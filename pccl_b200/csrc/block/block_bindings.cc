@@ -148,7 +148,7 @@ variable_list route_run(const RouteCall& c, const Tensor& logits, const OptTenso
   if (m.defined()) a.mask = reinterpret_cast<const uint8_t*>(m.const_data_ptr<bool>());
   // One allocation: an allocation costs the host as much as all of the arithmetic here costs the GPU for one token.
   const int64_t n = static_cast<int64_t>(a.tokens) * a.top_k, rest = (3 * n + a.experts + 1 + 3) / 4 * 4;
-  const int64_t bytes = static_cast<int64_t>(block::route_workspace(a.tokens, a.experts, a.top_k));
+  const int64_t bytes = static_cast<int64_t>(block::route_workspace(a));
   const Tensor all = fresh({rest + (bytes + 3) / 4}, at::kInt, logits);
   if (bytes) a.workspace = all.mutable_data_ptr<int32_t>() + rest;
   Tensor idx = slice_of(all.storage(), {a.tokens, a.top_k}, at::kInt, 0);

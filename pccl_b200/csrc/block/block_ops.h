@@ -36,7 +36,7 @@ struct RouteArgs {
   int32_t* offsets;           // [experts + 1]: first row of every expert
   void* workspace;            // route_workspace() bytes (null when that is 0)
 };
-size_t route_workspace(int tokens, int experts, int top_k);
+size_t route_workspace(const RouteArgs& a);
 void route_topk(const RouteArgs& a, cudaStream_t stream);
 
 // dlogits[tokens][experts] (contiguous) from dweights[tokens][top_k]; the choice itself is constant.

@@ -6,7 +6,7 @@
 //   w_k = scale * p_k / sum p  (or scale * p_k);
 //   rows[t][k] = offsets[idx] + number of earlier tokens that chose the same expert.
 //
-// Up to 8 experts one thread takes a token (16384 tokens, 8 experts: 19 us with a warp each); above that one warp,
+// With few experts one thread takes a token (by_threads() has the rule), else one warp,
 // expert e in lane e / NE, so that the lowest lane holds the lowest number and a tie is decided by the first set bit of
 // a ballot.  Scores are compared as unsigned keys of the same order (one redux.sync a round); a lane keeps its keys
 // sorted, so that a round costs the winner a shift.  Many tokens are bound by instructions, not by the 4 bytes a
@@ -23,6 +23,8 @@
 // per expert are summed by the second kernel in block order.
 #include <math.h>
 
+#include <algorithm>
+
 #include "../common/util.h"
 #include "../engine/cuda_driver.h"
 #include "vec.cuh"
@@ -34,7 +36,8 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMostThreads = 1024;
-constexpr int kThreadExperts = 8;             // up to so many experts a thread takes a token
+constexpr int kThreadExperts = 8;             // up to so many experts a thread takes a token,
+constexpr int kThreadExpertsFlat = 32;        // up to so many where the logits alone decide
 
 struct RouteParams {
   RouteArgs a;
@@ -700,16 +703,16 @@ __global__ void __launch_bounds__(kMost, 1) route_warp_kernel(const RouteParams 
 // ---- a thread per token ----------------------------------------------------------------------------------------
 // choose() by one thread over all experts; numbers go to picked[0 .. top_k - 1].  Returns whether the choice has to be
 // repeated in 64 bits.
-template <typename F, int NE>
-__device__ __forceinline__ bool choose_alone(const RouteParams& p, const F (&s)[NE], float tau, bool check,
-                                             const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+template <typename T, typename F, int NE>
+__device__ __forceinline__ bool choose_alone(const RouteParams& p, const T* row, const F (&s)[NE], float tau, bool check,
+                                             const float (&l)[NE], uint16_t* picked) {
   using Key = decltype(key_of(F()));
   const RouteArgs& a = p.a;
   Key key[NE];
 #pragma unroll
   for (int j = 0; j < NE; ++j) key[j] = j < a.experts ? key_of(s[j]) : Key(0);
   bool close = false;
-  if (a.top_groups < a.groups) {
+  if (NE <= kThreadExperts && a.top_groups < a.groups) {
     const int size = a.experts / a.groups;
     Key score[NE];                                 // of the group of each expert
 #pragma unroll
@@ -756,32 +759,30 @@ __device__ __forceinline__ bool choose_alone(const RouteParams& p, const F (&s)[
   for (int i = 0; i < rounds; ++i) {
     Key best = 0;
     int at = 0;
-    float l1 = 0.f, b1 = 0.f;
 #pragma unroll
     for (int j = 0; j < NE; ++j)
       if (key[j] > best) {
         best = key[j];
         at = j;
-        l1 = l[j];
-        b1 = bias[j];
       }
     if (best == 0) break;                          // only the runner-up can be missing
-    if (check && i > 0 && !(l0 == l1 && b0 == b1)) {
+    if (check) {
+      const float l1 = clean(to_f32<T>(row[at])), b1 = clean(a.bias[at]);
       const float a0 = static_cast<float>(value_of(before));
-      close |= !(a0 - static_cast<float>(value_of(best)) > tau + 0x1p-21f * fabsf(a0));
+      if (i > 0 && !(l0 == l1 && b0 == b1)) close |= !(a0 - static_cast<float>(value_of(best)) > tau + 0x1p-21f * fabsf(a0));
+      l0 = l1;
+      b0 = b1;
     }
     if (i < a.top_k) picked[i] = static_cast<uint16_t>(at);
 #pragma unroll
     for (int j = 0; j < NE; ++j)
       if (j == at) key[j] = 0;
     before = best;
-    l0 = l1;
-    b0 = b1;
   }
   return close;
 }
-template <int NE>
-__device__ __noinline__ void choose_alone_wide(const RouteParams& p, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
+template <typename T, int NE>
+__device__ __noinline__ void choose_alone_wide(const RouteParams& p, const T* row, const float (&l)[NE], const float (&bias)[NE], uint16_t* picked) {
   const RouteArgs& a = p.a;
   float top = -INFINITY;
 #pragma unroll
@@ -798,17 +799,22 @@ __device__ __noinline__ void choose_alone_wide(const RouteParams& p, const float
     if (!a.sigmoid && total > 0) s[j] /= total;
     s[j] = l[j] == -INFINITY || bias[j] == -INFINITY ? -INFINITY : s[j] + static_cast<double>(bias[j]);
   }
-  choose_alone<double, NE>(p, s, 0.f, false, l, bias, picked);
+  choose_alone<T, double, NE>(p, row, s, 0.f, false, l, picked);
 }
 
 template <typename T, int NE>
 __device__ __forceinline__ void load_token(const RouteParams& p, int64_t t, float (&l)[NE]) {
+  constexpr int kPiece = NE * sizeof(T) < 16 ? NE : 16 / static_cast<int>(sizeof(T));
   const RouteArgs& a = p.a;
   const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-  if (p.vec) {
-    const Share<T, NE> raw = *reinterpret_cast<const Share<T, NE>*>(row);
+  if (p.vec) {                                     // whole pieces, as many as there are experts
 #pragma unroll
-    for (int j = 0; j < NE; ++j) l[j] = clean(to_f32<T>(raw.v[j]));
+    for (int i = 0; i < NE; i += kPiece) {
+      Share<T, kPiece> raw = empty_share<T, kPiece>();
+      if (i < a.experts) raw = *reinterpret_cast<const Share<T, kPiece>*>(row + i);
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j) l[i + j] = clean(to_f32<T>(raw.v[j]));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < NE; ++j) l[j] = j < a.experts ? clean(to_f32<T>(row[j])) : -INFINITY;
@@ -816,7 +822,7 @@ __device__ __forceinline__ void load_token(const RouteParams& p, int64_t t, floa
 }
 
 template <typename T, int NE>
-__global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(NE <= 8 ? kMostThreads : 256, 1) route_thread_kernel(const RouteParams p) {
   extern __shared__ __align__(16) uint32_t smem[];
   const RouteArgs& a = p.a;
   const BlockRows mine(p, smem);
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
   const int count = min(p.tokens_per_block, a.tokens - first);
   asm volatile("griddepcontrol.launch_dependents;");
   mine.clear(p);
-  const bool scored = a.bias != nullptr || (a.top2 && a.top_groups < a.groups);
+  const bool scored = NE <= kThreadExperts && (a.bias != nullptr || (a.top2 && a.top_groups < a.groups));
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += blockDim.x) {
     const int64_t t = first + i;
@@ -837,7 +843,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
       load_token<T, NE>(p, t, l);
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
-        bias[j] = a.bias ? clean(a.bias[min(j, a.experts - 1)]) : 0.f;
+        bias[j] = NE <= kThreadExperts && a.bias ? clean(a.bias[min(j, a.experts - 1)]) : 0.f;
         s[j] = l[j];
       }
       if (!a.sigmoid && (scored || !a.renormalise)) {
@@ -851,20 +857,20 @@ __global__ void __launch_bounds__(kMostThreads, 1) route_thread_kernel(const Rou
           total += s[j];
         }
       }
-      if (scored) {
+      if (NE <= kThreadExperts && scored) {
         const float inv = total > 0.f ? 1.f / total : 0.f;
 #pragma unroll
         for (int j = 0; j < NE; ++j) {
           const float prob = a.sigmoid ? quick_sigmoid(l[j]) : s[j] * inv;
           s[j] = l[j] == -INFINITY ? -INFINITY : prob + bias[j];
         }
-        if (choose_alone<float, NE>(p, s, score_error(a.sigmoid, NE, inv), true, l, bias, picked))
+        if (choose_alone<T, float, NE>(p, row, s, score_error(a.sigmoid, NE, inv), true, l, picked))
           out_of_line(l, bias, [&](const float (&l1)[NE], const float (&b1)[NE]) {
-            choose_alone_wide<NE>(p, l1, b1, picked);
+            choose_alone_wide<T, NE>(p, row, l1, b1, picked);
             return 0;
           });
       } else {
-        choose_alone<float, NE>(p, l, 0.f, false, l, bias, picked);
+        choose_alone<T, float, NE>(p, row, l, 0.f, false, l, picked);
       }
     }
     float best = -INFINITY, sum = 0.f;
@@ -1071,15 +1077,19 @@ __global__ void __launch_bounds__(128) route_thread_backward_kernel(const RouteP
     for (int j = 0; j < NE; ++j) d[j] = l[j] == -INFINITY ? 0.f : a.scale * d[j] * sigmoid(l[j]) * sigmoid(-l[j]);
   }
   T* row = static_cast<T*>(p.dlogits) + t * a.experts;
-  Share<T, NE> out;
-#pragma unroll
-  for (int j = 0; j < NE; ++j) out.v[j] = from_f32<T>(d[j]);
+  constexpr int kPiece = NE * sizeof(T) < 16 ? NE : 16 / static_cast<int>(sizeof(T));
   if (p.vec) {
-    *reinterpret_cast<Share<T, NE>*>(row) = out;
+#pragma unroll
+    for (int i = 0; i < NE; i += kPiece) {
+      Share<T, kPiece> out;
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j) out.v[j] = from_f32<T>(d[i + j]);
+      if (i < a.experts) *reinterpret_cast<Share<T, kPiece>*>(row + i) = out;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < NE; ++j)
-      if (j < a.experts) row[j] = out.v[j];
+      if (j < a.experts) row[j] = from_f32<T>(d[j]);
   }
 }
 
@@ -1092,9 +1102,16 @@ size_t route_smem(int experts, int top_k, int tokens_per_block) {
 }
 
 // Experts of a lane (or of a thread) that the kernels are compiled for.
-int share_of(int experts) {
-  if (experts <= kThreadExperts) return experts <= 4 ? 4 : 8;
-  const int ne = (experts + 31) / 32;
+// A thread per token or a warp per token.  Measured, thread / warp: 8 experts top 2, 16384 tokens 7.5 / 14.6 us, one token
+// 4.1 / 3.3; 16 experts top 2, 16384 tokens 7.9 / 14.6, top 8 with 4096 tokens 12.9 / 10.1, 256 tokens 5.8 / 6.6.  With a bias a
+// thread that has to choose again in 64 bits over all of 32 experts holds up its warp for 20 us.
+bool by_threads(const RouteArgs& a) {
+  if (a.experts <= kThreadExperts) return a.tokens > 8;
+  return a.experts <= kThreadExpertsFlat && a.top_groups == a.groups && a.bias == nullptr && a.top_k <= 4 && a.tokens > 1024;
+}
+int share_of(const RouteArgs& a) {
+  if (by_threads(a)) return a.experts <= 4 ? 4 : a.experts <= 8 ? 8 : a.experts <= 16 ? 16 : 32;
+  const int ne = (a.experts + 31) / 32;
   return ne <= 6 ? ne : ne <= 8 ? 8 : ne <= 16 ? 16 : 32;
 }
 // Lanes that share a group where a lane has `ne` experts, if groups fall into whole lanes, a power of two of them.
@@ -1105,19 +1122,19 @@ int lanes_of(const RouteArgs& a, int ne) {
 
 // Few tokens stay in one block, which needs no second kernel; more get about a block per SM, small ones as long as
 // there are SMs left (256 tokens of 256 experts: 32 a block 22.6 us, 8 a block 17).
-int tokens_per_block(int tokens, int experts, int top_k) {
+int tokens_per_block(const RouteArgs& a) {
   int tpb;
-  if (experts <= kThreadExperts) {
-    tpb = tokens <= 1024 ? tokens : (tokens + 591) / 592;
-    if (tpb < 128 && tokens > 1024) tpb = 128;
+  if (by_threads(a)) {
+    tpb = a.tokens <= 256 ? a.tokens : (a.tokens + 591) / 592;
+    if (tpb < 128 && a.tokens > 256) tpb = 128;
     if (tpb > 1024) tpb = 1024;
   } else {
-    tpb = tokens <= 24 ? tokens : (tokens + 147) / 148;
+    tpb = a.tokens <= 24 ? a.tokens : (a.tokens + 147) / 148;
     if (tpb < 8) tpb = 8;
   }
   if (tpb > 32) tpb = (tpb + 31) / 32 * 32;
   if (tpb < 1) tpb = 1;
-  while (tpb > 32 && route_smem(experts, top_k, tpb) > kMaxRouteSmem) tpb -= 32;
+  while (tpb > 32 && route_smem(a.experts, a.top_k, tpb) > kMaxRouteSmem) tpb -= 32;
   return tpb;
 }
 
@@ -1150,14 +1167,14 @@ void launch_warps(const RouteParams& p, bool backward, int blocks, size_t smem, 
 template <typename T, int NE>
 void launch_threads(const RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
   if (backward) route_thread_backward_kernel<T, NE><<<(p.a.tokens + 127) / 128, 128, 0, stream>>>(p);
-  else launch_route(route_thread_kernel<T, NE>, p, blocks, p.tokens_per_block < 128 ? 128 : p.tokens_per_block, smem, stream);
+  else launch_route(route_thread_kernel<T, NE>, p, blocks, std::clamp(p.tokens_per_block, 128, NE <= 8 ? kMostThreads : 256), smem, stream);
 }
 
 void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStream_t stream) {
   const RouteArgs& a = p.a;
-  const bool alone = a.experts <= kThreadExperts;
+  const bool alone = by_threads(a);
   const int bytes = dtype_bytes(a.dtype);
-  int ne = share_of(a.experts);
+  int ne = share_of(a);
   p.lanes = lanes_of(a, ne);
   // A few idle lanes are cheaper than groups that cross them.
   if (!alone && a.top_groups < a.groups)
@@ -1167,12 +1184,14 @@ void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStre
         if (p.lanes) ne = wider;
       }
   const int piece = ne * bytes < 16 ? ne * bytes : 16;
-  p.vec = power_of_two(ne) && (alone ? a.experts == ne : a.experts % ne == 0) &&
+  p.vec = power_of_two(ne) && (alone ? a.experts * bytes % piece == 0 : a.experts % ne == 0) &&
           reinterpret_cast<uintptr_t>(a.logits) % piece == 0 && a.ld * bytes % piece == 0 &&
           (!backward || (reinterpret_cast<uintptr_t>(p.dlogits) % piece == 0 && static_cast<int64_t>(a.experts) * bytes % piece == 0));
   PCCL_BLOCK_TYPES(a.dtype, T,
     if (alone && ne == 4) launch_threads<T, 4>(p, backward, blocks, smem, stream);
-    else if (alone) launch_threads<T, 8>(p, backward, blocks, smem, stream);
+    else if (alone && ne == 8) launch_threads<T, 8>(p, backward, blocks, smem, stream);
+    else if (alone && ne == 16) launch_threads<T, 16>(p, backward, blocks, smem, stream);
+    else if (alone) launch_threads<T, 32>(p, backward, blocks, smem, stream);
     else if (ne == 1) launch_warps<T, 1>(p, backward, blocks, smem, stream);
     else if (ne == 2) launch_warps<T, 2>(p, backward, blocks, smem, stream);
     else if (ne == 3) launch_warps<T, 3>(p, backward, blocks, smem, stream);
@@ -1187,16 +1206,16 @@ void launch_any(RouteParams& p, bool backward, int blocks, size_t smem, cudaStre
 
 }  // namespace
 
-size_t route_workspace(int tokens, int experts, int top_k) {
-  const int tpb = tokens_per_block(tokens, experts, top_k);
-  const int blocks = (tokens + tpb - 1) / tpb;
-  return blocks > 1 ? static_cast<size_t>(blocks) * ((experts + 3) / 4 * 4) * sizeof(uint16_t) : 0;
+size_t route_workspace(const RouteArgs& a) {
+  const int tpb = tokens_per_block(a);
+  const int blocks = (a.tokens + tpb - 1) / tpb;
+  return blocks > 1 ? static_cast<size_t>(blocks) * ((a.experts + 3) / 4 * 4) * sizeof(uint16_t) : 0;
 }
 
 void route_topk(const RouteArgs& a, cudaStream_t stream) {
   RouteParams p{};
   p.a = a;
-  p.tokens_per_block = tokens_per_block(a.tokens, a.experts, a.top_k);
+  p.tokens_per_block = tokens_per_block(a);
   p.words = (p.tokens_per_block + 31) / 32;
   p.pitch = (a.experts + 3) / 4 * 4;
   p.per_choice = static_cast<uint32_t>((0x100000000ull + a.top_k - 1) / a.top_k);
