@@ -165,9 +165,9 @@ __device__ __forceinline__ void fetch_share(char* image, const T* row, const Col
 
 // Bytes of a window for any row of T.
 template <typename T> __host__ __device__ constexpr int window_bytes(int threads) { return threads * kBytes<T> + 16; }
-// The 16-byte blocks that cover the block's part of the row, and zeros up to the last column that a thread holds.  The first may begin with
-// values in front of it: such a block holds a value of the row, and allocations begin at multiples of 256
-// bytes, so all of it is theirs.  Nothing is read behind the row.
+// The 16-byte blocks that cover the block's part of the row, and zeros up to the last column that a thread holds.
+// The first may begin with values in front of it: such a block holds a value of the row, and allocations begin at
+// multiples of 256 bytes, so all of it is theirs.  Nothing is read behind the row.
 template <typename T, int G>
 __device__ __forceinline__ void fetch_window(char* window, const T* row, const Columns<false, G>& c) {
   const uintptr_t begin = reinterpret_cast<uintptr_t>(row + c.part);

@@ -141,19 +141,20 @@ __device__ __forceinline__ int group_rank(int groups, int lanes, int group, Key 
   return rank;
 }
 
-// Whether all that is close is a pair of choices with equal logits and equal biases, which no arithmetic can part.
+// Whether all that is close are pairs of choices with equal logits and equal biases, which no arithmetic can part.  (A
+// choice and a runner-up that are equal are not enough: what stands behind them may be close to both.)
 template <typename T>
 __device__ __forceinline__ bool truly_tied(const RouteParams& p, int64_t t, int close, int pick) {
   const RouteArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   float l = 0.f, b = 0.f;
-  if (lane <= a.top_k && lane < a.experts) {
+  if (lane < a.top_k) {
     const int e = min(max(pick, 0), a.experts - 1);
     l = to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + e]);
     b = a.bias != nullptr ? a.bias[e] : 0.f;
   }
   const float l1 = __shfl_down_sync(kAll, l, 1), b1 = __shfl_down_sync(kAll, b, 1);
-  return !__any_sync(kAll, (close & 2) || ((close & 1) && !(l == l1 && b == b1)));
+  return !__any_sync(kAll, (close & 2) || ((close & 1) && !(lane < a.top_k - 1 && l == l1 && b == b1)));
 }
 
 // A warp's shared memory: the lanes' sorted keys, one above the other, and what was picked.
@@ -174,8 +175,8 @@ template <int NE> struct Deck {
 // (a round of 65536 tokens took 3.7 us with the keys shifted in registers, 2.7 so).
 //
 // Where neighbours of the choice are close, the choices and the runner-up are ranked again by 64-bit scores, a lane
-// each: enough unless something behind the runner-up is close to it as well, is not its equal in logit and bias, or
-// the scores need the whole row's sum.  Returns whether the choice has to be repeated over all experts.
+// each: enough unless something behind the runner-up is close to it as well and is not its equal in logit and bias (or is,
+// and the runner-up passes more than one choice), or the scores need the whole row's sum.  Returns whether the choice has to be repeated over all experts.
 template <typename T, int NE>
 __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, const float (&s)[NE], float tau, bool exact,
                                              const float (&l)[NE], const float (&bias)[NE], Deck<NE>& deck, int* pick) {
@@ -227,8 +228,10 @@ __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, co
   }
   __syncwarp();
   const uint2 won = deck.won[lane];
-  const bool there = lane < rounds && won.x > 7u;            // a runner-up can be missing
-  *pick = there ? static_cast<int>(won.y >> 3) * NE + static_cast<int>(~won.y & 7u) : -1;
+  // A runner-up can be missing, or be a place behind the last expert.
+  const int number = static_cast<int>(won.y >> 3) * NE + static_cast<int>(~won.y & 7u);
+  const bool there = lane < rounds && won.x > 7u && number < a.experts;
+  *pick = there ? number : -1;
   if (exact) return false;
   if (a.bias == nullptr) tau = 0.f;                          // ranked by logits
   // Scores nearer than this may stand the other way round.  (Keys lose up to seven units, all in one direction.)
@@ -236,17 +239,18 @@ __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, co
   const uint32_t below = __shfl_down_sync(kAll, won.x, 1);
   const float score = value_of(won.x);
   const bool close = lane < a.top_k && below > 7u && !(score - value_of(below) > reach(score));
-  if (again || !__any_sync(kAll, close)) return again;
-  if (a.bias != nullptr && !a.sigmoid) return !truly_tied<T>(p, t, close ? 1 : 0, *pick);
+  const unsigned pairs = __ballot_sync(kAll, close);
+  if (again || pairs == 0) return again;
 
   float le = 0.f, be = 0.f;
   if (there) {
     le = clean(to_f32<T>(static_cast<const T*>(a.logits)[t * a.ld + *pick]));
     be = a.bias ? clean(a.bias[*pick]) : 0.f;
   }
-  const uint32_t next = warp_max(top | 7u), last = __shfl_sync(kAll, won.x, a.top_k);
-  const float edge = value_of(last);
-  if (last > 7u && next > 7u && !(edge - value_of(next) > reach(edge))) {
+  const uint32_t next = warp_max(top | 7u);
+  const float edge = value_of(__shfl_sync(kAll, won.x, a.top_k));
+  const bool more = (pairs >> (a.top_k - 1)) & 1u && next > 7u && !(edge - value_of(next) > reach(edge));
+  if (more) {
     // Something behind the runner-up is close to it.  Only its equals may be: all that reaches it and is not its
     // equal has to be among the choices.
     const float lr = __shfl_sync(kAll, le, a.top_k), br = __shfl_sync(kAll, be, a.top_k);
@@ -259,6 +263,10 @@ __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, co
     const unsigned chosen = __ballot_sync(kAll, lane < a.top_k && !(le == lr && be == br));
     if (others != __popc(chosen)) return true;
   }
+  if (a.bias != nullptr && !a.sigmoid) {           // 64-bit scores need the row's sum, but equals need none
+    const float l1 = __shfl_down_sync(kAll, le, 1), b1 = __shfl_down_sync(kAll, be, 1);
+    return __any_sync(kAll, close && !(le == l1 && be == b1));
+  }
   double wide = a.bias == nullptr ? static_cast<double>(le) : 1.0 / (1.0 + exp(-static_cast<double>(le))) + static_cast<double>(be);
   if (le == -INFINITY || be == -INFINITY || !there) wide = -INFINITY;
   int rank = 0;
@@ -267,6 +275,8 @@ __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, co
     const int e = __shfl_sync(kAll, *pick, i);
     if (e >= 0) rank += other > wide || (other == wide && e < *pick) ? 1 : 0;
   }
+  // A runner-up that passes more than one choice would take its equals along.
+  if (more && __shfl_sync(kAll, rank, a.top_k) < a.top_k - 1) return true;
   if (there) deck.picked[rank] = static_cast<uint16_t>(*pick);
   __syncwarp();
   if (there) *pick = deck.picked[lane];
@@ -769,7 +779,14 @@ __device__ __forceinline__ bool choose_alone(const RouteParams& p, const T* row,
     if (check) {
       const float l1 = clean(to_f32<T>(row[at])), b1 = clean(a.bias[at]);
       const float a0 = static_cast<float>(value_of(before));
-      if (i > 0 && !(l0 == l1 && b0 == b1)) close |= !(a0 - static_cast<float>(value_of(best)) > tau + 0x1p-21f * fabsf(a0));
+      const bool tied = l0 == l1 && b0 == b1;
+      if (i > 0 && !tied) close |= !(a0 - static_cast<float>(value_of(best)) > tau + 0x1p-21f * fabsf(a0));
+      if (i > 0 && i == a.top_k && tied) {         // what stands behind the runner-up must not be close, but for its equals
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+          if (key[j] != 0 && !(a0 - static_cast<float>(value_of(key[j])) > tau + 0x1p-21f * fabsf(a0)))
+            close |= !(l[j] == l1 && clean(a.bias[min(j, a.experts - 1)]) == b1);
+      }
       l0 = l1;
       b0 = b1;
     }

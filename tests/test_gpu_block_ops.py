@@ -159,6 +159,35 @@ def test_route_ranks_near_pairs_again(scoring, experts):
     _check_route(near, k, scoring=scoring, groups=4, top_groups=2)
 
 
+@pytest.mark.parametrize("experts", [8, 24, 40, 64, 200, 256, 500])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_ranks_a_few_near_ones_among_many(experts, biased):
+    """Two to seven experts a row within eight units of the last place, some equal, around the end of the choice; the
+    rest far below."""
+    g = _gen(15)
+    tokens = 3000
+    logits = _normal(g, tokens, experts) - 8
+    few = torch.randint(2, 8, (tokens, 1), device="cuda", generator=g)
+    where = torch.rand(tokens, experts, device="cuda", generator=g).argsort(-1) < few
+    steps = torch.randint(0, 8, (tokens, experts), device="cuda", generator=g)
+    logits = torch.where(where, 1 + steps * 2.0 ** -23, logits)
+    bias = torch.zeros(experts, device="cuda") if biased else None
+    for k in (1, 2, 3, 4):
+        _check_route(logits, k, bias=bias, scoring="sigmoid", grad=False)
+        _check_route(logits, k, bias=bias, scoring="softmax", grad=False)
+
+
+def test_route_of_all_experts_that_are_all_out():
+    """As many choices as experts, none of them live: nothing behind the last expert is touched."""
+    for experts, k in ((31, 31), (9, 9), (5, 5), (33, 31)):
+        logits = torch.full((40, experts), -math.inf, device="cuda")
+        logits[::2, 0] = 1.0
+        for bias in (None, torch.zeros(experts, device="cuda")):
+            got = route_topk(logits, k, bias=bias, scoring="sigmoid")
+            assert torch.equal(got.idx.long(), torch.arange(k, device="cuda").expand(40, k))
+            assert bool((got.weights[1::2] == 0).all()) and bool((got.weights[::2, 0] == 1).all())
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalise", [True, False])
 @pytest.mark.parametrize("biased", [False, True])
