@@ -20,6 +20,10 @@ their own, on ordinary tensors of one GPU and with gradients:
 ``route_topk``   scores (softmax or sigmoid, a bias for balance, groups), top-k, weights, expert order;
 ``dispatch``     token rows into expert order, one copy per choice;
 ``combine``      the experts' rows back to their tokens, weighted and summed.
+
+They run on the tensors' device and its current stream, may be captured into a CUDA graph (a backward pass, as for any
+torch operator, only while no eager graph of the same leaves is alive), and raise ``ValueError`` for arguments they do
+not take.
 """
 
 from __future__ import annotations
@@ -192,7 +196,7 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
     chosen only where nothing else is left, and then with weight 0.  Plus infinity counts as the largest finite
     logit.  Tokens where ``mask`` (bool ``[tokens]``) is false choose nothing: index and row -1, weight 0.
 
-    Up to 1024 experts, 32 groups and 31 choices.  ``weights`` carries the gradient of ``logits`` (once: it cannot
+    Up to 1024 experts, 32 groups and 31 choices.  The four results share one allocation.  ``weights`` carries the gradient of ``logits`` (once: it cannot
     be differentiated twice); the order of the choices within an expert is that of the tokens, on every run.
     """
     if scoring not in ("softmax", "sigmoid"):

@@ -4,7 +4,9 @@
 ``residual_rms_norm``   what stands between two blocks of a residual stream, in one pass over its rows:
                         the norm behind a block, its gate, the residual sum and the norm before the next block.
 
-``pccl_b200.ops.AllReduceResidualRMSNorm`` is the form for partial outputs that are first summed over ranks.
+They run on the tensors' device and its current stream, may be captured into a CUDA graph (a backward pass, as for any
+torch operator, only while no eager graph of the same leaves is alive), and raise ``ValueError`` for arguments they do
+not take.  ``pccl_b200.ops.AllReduceResidualRMSNorm`` is the form for partial outputs that are first summed over ranks.
 The reference has no norm operator.
 """
 
