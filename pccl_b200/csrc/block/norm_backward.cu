@@ -368,7 +368,7 @@ void backward_mode(NormParams& p, bool vec, cudaStream_t stream) {
   else launch(norm_backward_kernel<TX, TR, kWindow, kFull, false>, p, l, stream);
 }
 
-// Calls f.template operator()<TX, TR, kFull>() for the types and weights of these arguments.
+// Calls f(TX(), TR(), kFull) for the types and weights of these arguments.
 template <class F> void with_types(const NormArgs& a, F f) {
   PCCL_BLOCK_TYPES(a.xt, T,
     if (a.rt == a.xt && has_g1(a)) f(T(), T(), std::true_type());
