@@ -224,16 +224,23 @@ variable_list route_topk(const Tensor& logits, int64_t top_k, const OptTensor& b
 }
 
 // ---- dispatch / combine ----------------------------------------------------------------------------------
-block::MoveArgs move_args(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+block::MoveArgs move_args(const Tensor& x, const Tensor& rows) {
   block::MoveArgs a{};
   a.dtype = dtype_of(x);
   a.tokens = static_cast<int>(rows.size(0));
   a.top_k = static_cast<int>(rows.size(1));
   a.hidden = static_cast<int>(x.size(1));
-  a.experts = static_cast<int>(offsets.size(0) - 1);
   a.rows = rows.const_data_ptr<int32_t>();
-  a.offsets = offsets.const_data_ptr<int32_t>();
   return a;
+}
+
+// Memory for finding the rows that no choice names; null where none is needed.
+Tensor move_space(block::MoveArgs& a, const Tensor& like) {
+  const size_t bytes = block::move_workspace(a);
+  if (bytes == 0) return Tensor();
+  Tensor space = fresh({static_cast<int64_t>(bytes / 4)}, at::kInt, like);
+  a.workspace = space.mutable_data_ptr<int32_t>();
+  return space;
 }
 
 void check_move(const char* op, const Tensor& x, const Tensor& rows, const Tensor& offsets) {
@@ -246,18 +253,20 @@ void check_move(const char* op, const Tensor& x, const Tensor& rows, const Tenso
   PCCL_ARG(x.size(1) >= 1 && x.size(1) <= (1 << 24), op << ": rows hold at least one value and at most 2^24");
 }
 
-Tensor dispatch_run(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+Tensor dispatch_run(const Tensor& x, const Tensor& rows) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Rows src = as_rows(x);
+  block::MoveArgs a = move_args(x, rows);
   Tensor out = fresh({rows.numel(), x.size(1)}, x.scalar_type(), x);
-  block::dispatch_rows(move_args(x, rows, offsets), src.ptr(), src.ld, out.mutable_data_ptr(), stream_of(x));
+  const Tensor space = move_space(a, x);
+  block::dispatch_rows(a, src.ptr(), src.ld, out.mutable_data_ptr(), stream_of(x));
   return out;
 }
 
-Tensor combine_run(const Tensor& y, const Tensor& weights, const Tensor& rows, const Tensor& offsets) {
+Tensor combine_run(const Tensor& y, const Tensor& weights, const Tensor& rows) {
   const c10::cuda::CUDAGuard guard(y.device());
   const Rows src = as_rows(y);
-  block::MoveArgs a = move_args(y, rows, offsets);
+  block::MoveArgs a = move_args(y, rows);
   if (weights.defined()) a.weights = weights.const_data_ptr<float>();
   Tensor out = fresh({rows.size(0), y.size(1)}, y.scalar_type(), y);
   block::combine_rows(a, src.ptr(), src.ld, out.mutable_data_ptr(), stream_of(y));
@@ -265,18 +274,18 @@ Tensor combine_run(const Tensor& y, const Tensor& weights, const Tensor& rows, c
 }
 
 struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rows) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({rows, offsets});
-    return dispatch_run(x, rows, offsets);
+    ctx->save_for_backward({rows});
+    return dispatch_run(x, rows);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list result(3);
+    variable_list result(2);
     if (!grads[0].defined()) return result;
     const auto saved = ctx->get_saved_variables();
     {
       at::NoGradGuard no_grad;
-      result[0] = combine_run(grads[0], Tensor(), saved[0], saved[1]);
+      result[0] = combine_run(grads[0], Tensor(), saved[0]);
     }
     once(result);
     return result;
@@ -284,24 +293,27 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
 };
 
 struct CombineFunction : torch::autograd::Function<CombineFunction> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor& rows,
-                        const Tensor& offsets) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& weights, const Tensor& rows) {
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({y, weights, rows, offsets});
-    return combine_run(y, weights, rows, offsets);
+    ctx->save_for_backward({y, weights, rows});
+    return combine_run(y, weights, rows);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list result(4);
+    variable_list result(3);
     if (!grads[0].defined()) return result;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &y = saved[0], &weights = saved[1], &rows = saved[2], &offsets = saved[3];
+    const Tensor &y = saved[0], &weights = saved[1], &rows = saved[2];
     {
       at::NoGradGuard no_grad;
       const c10::cuda::CUDAGuard guard(y.device());
       const Rows src = as_rows(y), d = as_rows(grads[0]);
-      block::MoveArgs a = move_args(y, rows, offsets);
+      block::MoveArgs a = move_args(y, rows);
       a.weights = weights.const_data_ptr<float>();
-      if (ctx->needs_input_grad(0)) result[0] = fresh(y.sizes(), y.scalar_type(), y);
+      Tensor space;
+      if (ctx->needs_input_grad(0)) {
+        result[0] = fresh(y.sizes(), y.scalar_type(), y);
+        space = move_space(a, y);
+      }
       if (ctx->needs_input_grad(1)) result[1] = fresh(weights.sizes(), at::kFloat, y);
       block::combine_rows_backward(a, src.ptr(), src.ld, d.ptr(), d.ld,
                                    result[0].defined() ? result[0].mutable_data_ptr() : nullptr,
@@ -319,8 +331,8 @@ Tensor dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
   on_device(x, x, op, "x");
   on_device(rows, x, op, "routing.rows");
   on_device(offsets, x, op, "routing.offsets");
-  if (at::GradMode::is_enabled() && x.requires_grad()) return DispatchFunction::apply(x, rows, offsets);
-  return dispatch_run(x, rows, offsets);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return DispatchFunction::apply(x, rows);
+  return dispatch_run(x, rows);
 }
 
 Tensor combine(const Tensor& y, const Tensor& weights, const Tensor& rows, const Tensor& offsets) {
@@ -334,8 +346,8 @@ Tensor combine(const Tensor& y, const Tensor& weights, const Tensor& rows, const
   on_device(rows, y, op, "routing.rows");
   on_device(offsets, y, op, "routing.offsets");
   if (at::GradMode::is_enabled() && (y.requires_grad() || weights.requires_grad()))
-    return CombineFunction::apply(y, weights, rows, offsets);
-  return combine_run(y, weights, rows, offsets);
+    return CombineFunction::apply(y, weights, rows);
+  return combine_run(y, weights, rows);
 }
 
 // ---- norms -------------------------------------------------------------------------------------------------

@@ -43,18 +43,22 @@ void route_topk(const RouteArgs& a, cudaStream_t stream);
 void route_topk_backward(const RouteArgs& a, const float* dweights, void* dlogits, cudaStream_t stream);
 
 // ---- rows into expert order and back ---------------------------------------------------------------
-struct MoveArgs {
+// What follows these in a kernel's parameters begins at 16 bytes: combine of 1777 x 1431 fp16 takes 10.9 us instead of 10.3
+// where it does not.
+struct alignas(16) MoveArgs {
   DType dtype;
-  int tokens, top_k, hidden, experts;
-  const int32_t* rows;        // [tokens][top_k]; a value outside [0, tokens * top_k) moves nothing
-  const int32_t* offsets;     // [experts + 1]; rows from offsets[experts] on hold no choice
+  int tokens, top_k, hidden;
+  const int32_t* rows;        // [tokens][top_k], no two the same; a value outside [0, tokens * top_k) moves nothing
   const float* weights;       // [tokens][top_k] (combine)
+  void* workspace;            // move_workspace() bytes (null when that is 0), where rows that no choice names are cleared
 };
-// out[rows[t][k]] = x[t]; rows behind the last choice become zero.
+size_t move_workspace(const MoveArgs& a);
+// out[rows[t][k]] = x[t]; rows that no choice names become zero.
 void dispatch_rows(const MoveArgs& a, const void* x, int64_t ldx, void* out, cudaStream_t stream);
 // out[t] = sum_k w[t][k] * y[rows[t][k]] (w = 1 where a.weights is null).
 void combine_rows(const MoveArgs& a, const void* y, int64_t ldy, void* out, cudaStream_t stream);
-// dy[rows[t][k]] = w[t][k] * dout[t], dw[t][k] = <y[rows[t][k]], dout[t]>; either output may be null.
+// dy[rows[t][k]] = w[t][k] * dout[t] (rows that no choice names become zero), dw[t][k] = <y[rows[t][k]], dout[t]>; either
+// output may be null, and without dy no workspace is needed.
 void combine_rows_backward(const MoveArgs& a, const void* y, int64_t ldy, const void* dout, int64_t ldd, void* dy,
                            float* dw, cudaStream_t stream);
 

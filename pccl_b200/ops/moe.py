@@ -162,7 +162,11 @@ def route(x: torch.Tensor, wg: torch.Tensor):
 
 class Routing(NamedTuple):
     """What ``route_topk`` chose.  Rows ``offsets[e]`` to ``offsets[e + 1]`` of a batch in expert order belong to
-    expert ``e``, tokens in order; rows from ``offsets[-1]`` on are unused (there are some only with a mask)."""
+    expert ``e``, tokens in order; rows from ``offsets[-1]`` on are unused (there are some only with a mask).
+
+    A caller may leave choices out (experts of bounded capacity, say): ``routing._replace(rows=...)`` with -1, or any
+    number outside the batch, in their places.  No two choices may name the same row: which of them it then holds, or
+    takes its gradient from, is not defined."""
 
     idx: torch.Tensor       # [tokens, top_k] int32, best first; -1 for masked tokens
     weights: torch.Tensor   # [tokens, top_k] float32, differentiable
@@ -211,8 +215,9 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """``out[routing.rows[t, k]] = x[t]``: ``[tokens * top_k, hidden]`` in expert order, for the experts' products.
 
-    Rows from ``routing.offsets[-1]`` on become zero.  The gradient of ``x`` sums its copies in 32 bits.  ``x`` is
-    float32, float16 or bfloat16 ``[tokens, hidden]``, rows at any distance.
+    Rows that no choice names become zero: those from ``routing.offsets[-1]`` on, and those of choices that were left
+    out.  The gradient of ``x`` sums its copies in 32 bits.  ``x`` is float32, float16 or bfloat16 ``[tokens, hidden]``,
+    rows at any distance.
     """
     return _block_native().dispatch(x, routing.rows, routing.offsets)
 
@@ -221,6 +226,6 @@ def combine(y: torch.Tensor, routing: Routing) -> torch.Tensor:
     """``out[t] = sum_k routing.weights[t, k] * y[routing.rows[t, k]]``: the experts' rows back to their tokens.
 
     The sum is taken in 32 bits in the order of the choices and rounded once; a token without choices gets zeros.
-    Gradients go to ``y`` (zero in rows that no choice reads) and to ``routing.weights``.
+    Gradients go to ``y`` (zero in rows that no choice names) and to ``routing.weights``.
     """
     return _block_native().combine(y, routing.weights, routing.rows, routing.offsets)

@@ -1,0 +1,126 @@
+"""Routing, dispatch / combine and the block norms on the GPU where they can go wrong: choices that are left out.
+Tolerances as in test_gpu_block_ops.py; what is not rounded is compared bit by bit."""
+
+import math
+
+import pytest
+import torch
+
+from block_reference import HALF_STEP, TINY
+from pccl_b200.ops import Routing, combine, dispatch, route_topk
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def _normal(g, *shape):
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+# --------------------------------------------------------------------------------------- dispatch / combine
+def _leave_nan_behind(*sizes):
+    """Fills the memory that the next allocations of these sizes (in bytes) are made of with NaN."""
+    held = [torch.full((max(1, n // 4),), math.nan, device="cuda") for n in sizes for _ in range(3)]
+    torch.cuda.synchronize()
+    del held
+
+
+def _dropped(g, tokens, experts, top_k, capacity, live):
+    """A routing whose choices beyond `capacity` rows an expert are left out, as a layer with bounded experts does."""
+    mask = torch.rand(tokens, device="cuda", generator=g) < live if live < 1 else None
+    r = route_topk(_normal(g, tokens, experts), top_k, mask=mask)
+    place = r.rows - r.offsets[:-1][r.idx.clamp(min=0).long()]
+    rows = torch.where((r.idx >= 0) & (place < capacity), r.rows, -1).contiguous()
+    return Routing(r.idx, r.weights.detach().requires_grad_(True), rows, r.offsets)
+
+
+def _check_whole(x, y, routing):
+    """dispatch(x), the gradient of combine(y): every row, those that no choice names among them."""
+    rows, (t, k) = routing.rows.long(), routing.rows.shape
+    n, hidden = t * k, x.shape[1]
+    live = (rows >= 0) & (rows < n)
+    named = torch.zeros(n, dtype=torch.bool, device="cuda")
+    named[rows[live]] = True
+    want = torch.zeros(n, hidden, dtype=x.dtype, device="cuda")
+    want[rows[live]] = x[:, None].expand(t, k, hidden)[live]
+    nbytes = n * hidden * x.element_size()
+    _leave_nan_behind(nbytes)
+    out = dispatch(x, routing)
+    assert torch.equal(out, want), f"{int((out != want).any(-1).sum())} rows of {n}, {int(named.sum())} named"
+    y = y.detach().requires_grad_(True)
+    dout = _normal(_gen(1), t, hidden).to(y.dtype)
+    out = combine(y, routing)
+    _leave_nan_behind(nbytes)
+    dy, dw = torch.autograd.grad(out, (y, routing.weights), dout)
+    w = torch.where(live, routing.weights.detach().double(), 0.0)
+    wide = torch.zeros(n, hidden, dtype=torch.float64, device="cuda")
+    wide[rows[live]] = (w[..., None] * dout.double()[:, None])[live]
+    # one product in 32 bits, rounded once more to the type
+    off = (dy.double() - wide).abs()
+    assert bool((off <= HALF_STEP[y.dtype] * wide.abs() * (1 + 2 ** -10) + TINY[y.dtype] + 2 ** -24 * wide.abs()).all())
+    assert bool((dy[~named] == 0).all()) and bool((dw[~live] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,hidden,experts,top_k,capacity,live", [
+    (1, 64, 4, 1, 0, 1.0), (8, 4096, 8, 2, 1, 1.0), (64, 33, 8, 2, 9, 0.8), (500, 256, 16, 2, 40, 1.0),
+    (300, 1431, 8, 3, 70, 0.9), (1000, 1, 4, 1, 100, 1.0), (4000, 128, 8, 2, 700, 1.0), (4096, 511, 16, 4, 900, 0.5),
+    (9000, 2056, 8, 8, 8000, 1.0), (3000, 64, 8, 2, 0, 1.0)])
+def test_rows_of_left_out_choices_are_zero(tokens, hidden, experts, top_k, capacity, live, dtype):
+    g = _gen(tokens + hidden)
+    routing = _dropped(g, tokens, experts, top_k, capacity, live)
+    _check_whole(_normal(g, tokens, hidden).to(dtype), _normal(g, tokens * top_k, hidden).to(dtype), routing)
+
+
+def test_rows_named_from_elsewhere_leave_zeros():
+    """Row numbers outside the batch, and offsets that say something else than the rows: the rows alone count."""
+    g = _gen(3)
+    for tokens in (30, 3000):
+        r = route_topk(_normal(g, tokens, 8), 2)
+        rows = r.rows.clone()
+        rows[0, 0], rows[1, 1], rows[2, 0], rows[3, 0] = -7, 2 * tokens, 2 ** 31 - 1, -2 ** 31
+        for offsets in (r.offsets, torch.zeros_like(r.offsets), torch.full_like(r.offsets, 2 ** 31 - 1)):
+            routing = Routing(r.idx, r.weights.detach().requires_grad_(True), rows, offsets)
+            for hidden in (64, 33):
+                _check_whole(_normal(g, tokens, hidden), _normal(g, 2 * tokens, hidden), routing)
+
+
+def test_moves_captured_with_choices_left_out():
+    """Enough choices for the kernel that notes them, captured and replayed with other rows and other values."""
+    g = _gen(5)
+    r = [_dropped(g, 1500, 8, 2, c, 0.9) for c in (1000, 300, 50)]
+    rows, weights = r[0].rows.clone(), r[0].weights.detach().clone().requires_grad_(True)
+    x = _normal(g, 1500, 136).bfloat16().requires_grad_(True)
+
+    def step(x, weights, rows):
+        routing = Routing(r[0].idx, weights, rows, r[0].offsets)
+        out = dispatch(x, routing)
+        back = combine(out * 2, routing)
+        return (out.detach(), back.detach()) + torch.autograd.grad(back.float().square().sum(), (x, weights))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, weights, rows)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(x, weights, rows)
+    for new in r[1:] + r[:1]:
+        with torch.no_grad():
+            x.copy_(_normal(g, 1500, 136))
+            rows.copy_(new.rows)
+            weights.copy_(new.weights)
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = step(x.detach().clone().requires_grad_(True), weights.detach().clone().requires_grad_(True), rows.clone())
+        assert all(torch.equal(a, b) for a, b in zip(outs, fresh))
+        dead = torch.ones(3000, dtype=torch.bool, device="cuda")
+        dead[rows[rows >= 0].long()] = False
+        assert bool((outs[0][dead] == 0).all())
