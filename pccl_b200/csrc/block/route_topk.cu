@@ -141,6 +141,16 @@ __device__ __forceinline__ int group_rank(int groups, int lanes, int group, Key 
   return rank;
 }
 
+// Least and largest value that the exact score of a group can have, which is `score` in 32 bits: its parts, of sizes that
+// add up to `size`, are off by half of tau each and by their own roundings, which a sum that cancels does not lose.  A
+// part of minus infinity is exact, and the sum with it.
+__device__ __forceinline__ float least_score(float score, float size, float tau, float step) {
+  return fmaxf(score - fmaf(step, size, tau), -INFINITY);      // not a NaN
+}
+__device__ __forceinline__ float largest_score(float score, float size, float tau, float step) {
+  return fmaxf(score + fmaf(step, size, tau), -INFINITY);
+}
+
 // Whether all that is close are pairs of choices with equal logits and equal biases, which no arithmetic can part.  (A
 // choice and a runner-up that are equal are not enough: what stands behind them may be close to both.)
 template <typename T>
@@ -195,14 +205,17 @@ __device__ __forceinline__ bool choose_quick(const RouteParams& p, int64_t t, co
       b1 = larger(b1, o1);
     }
     const int group = lane >> (__ffs(p.lanes) - 1);
-    const uint32_t mine = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+    const float v1 = value_of(b1), v2 = a.top2 ? value_of(b2) : 0.f;
+    const uint32_t mine = a.top2 ? key_of(v1 + v2) : b1;
     const bool real = group < a.groups;
     const int rank = group_rank(a.groups, p.lanes, group, mine);     // by the whole warp
     kept = real && rank < a.top_groups;
     if (!exact) {
-      const float low = value_of(~warp_max(kept ? ~mine : 0u)), high = value_of(warp_max(real && !kept ? mine : 0u));
-      // Two scores each, whose keys lose up to seven units in one direction.
-      again = !(low - high > 2.f * tau + 0x1.4p-20f * fabsf(low) + 0x1p-140f);
+      // Parts: half a unit of rounding, up to seven upwards by the keys; half a unit more for the sum.
+      const float size = fabsf(v1) + fabsf(v2), score = value_of(mine), any = tau + 0x1p-140f;
+      const float low = value_of(~warp_max(kept ? ~key_of(least_score(score, size, any, 0x1.4p-20f)) : 0u));
+      const float high = value_of(warp_max(real && !kept ? key_of(largest_score(score, size, any, 0x1p-22f)) : 0u));
+      again = !(low > high);
     }
     if (a.top2 && a.bias == nullptr) {             // the groups by their sums, the experts by their logits
 #pragma unroll
@@ -303,6 +316,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
   if (grouped) {
     const int size = a.experts / a.groups;
     Key mine = 0;                                  // the score of group `group`
+    F size_of = 0;                                 // and the sizes of its parts together
     int group = lane;
     if (p.lanes) {
       // A group is p.lanes neighbouring lanes.
@@ -318,7 +332,9 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
         b1 = larger(b1, o1);
       }
       group = lane / p.lanes;
-      mine = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+      const F v1 = value_of(b1), v2 = a.top2 ? value_of(b2) : F(0);
+      mine = a.top2 ? key_of(v1 + v2) : b1;
+      size_of = fabs(v1) + fabs(v2);
     } else {
       for (int g = 0; g < a.groups; ++g) {
         Key b1 = 0, b2 = 0;
@@ -332,19 +348,25 @@ __device__ __forceinline__ int choose(const RouteParams& p, const F (&s)[NE], fl
         }
         const Key m1 = warp_max(b1);
         Key score = m1;
+        F v2 = 0;
         if (a.top2) {
           const int owner = __ffs(__ballot_sync(kAll, b1 == m1)) - 1;
-          score = key_of(value_of(m1) + value_of(warp_max(lane == owner ? b2 : b1)));
+          v2 = value_of(warp_max(lane == owner ? b2 : b1));
+          score = key_of(value_of(m1) + v2);
         }
-        if (lane == g) mine = score;
+        if (lane == g) {
+          mine = score;
+          size_of = fabs(value_of(m1)) + fabs(v2);
+        }
       }
     }
     const int rank = group_rank(a.groups, p.lanes ? p.lanes : 1, group, mine);
     const bool kept = group < a.groups && rank < a.top_groups;
     if (check) {
-      const F low = value_of(static_cast<Key>(~warp_max(kept ? static_cast<Key>(~mine) : Key(0))));
-      const F high = value_of(warp_max(group < a.groups && !kept ? mine : Key(0)));
-      if (!(static_cast<float>(low - high) > 2.f * tau + 0x1p-20f * fabsf(static_cast<float>(low)))) close = 2;
+      const float score = static_cast<float>(value_of(mine)), size = static_cast<float>(size_of);
+      const float low = value_of(~warp_max(kept ? ~key_of(least_score(score, size, tau, 0x1p-22f)) : 0u));
+      const float high = value_of(warp_max(group < a.groups && !kept ? key_of(largest_score(score, size, tau, 0x1p-22f)) : 0u));
+      if (!(low > high)) close = 2;
     }
     if (p.lanes) {
 #pragma unroll
@@ -725,6 +747,7 @@ __device__ __forceinline__ bool choose_alone(const RouteParams& p, const T* row,
   if (NE <= kThreadExperts && a.top_groups < a.groups) {
     const int size = a.experts / a.groups;
     Key score[NE];                                 // of the group of each expert
+    F size_of[NE];                                 // and the sizes of its parts together
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       Key b1 = 0, b2 = 0;
@@ -734,9 +757,11 @@ __device__ __forceinline__ bool choose_alone(const RouteParams& p, const T* row,
           b2 = larger(b2, smaller(b1, key[i]));
           b1 = larger(b1, key[i]);
         }
-      score[j] = a.top2 ? key_of(value_of(b1) + value_of(b2)) : b1;
+      const F v1 = value_of(b1), v2 = a.top2 ? value_of(b2) : F(0);
+      score[j] = a.top2 ? key_of(v1 + v2) : b1;
+      size_of[j] = fabs(v1) + fabs(v2);
     }
-    Key low = ~Key(0), high = 0;
+    float low = INFINITY, high = -INFINITY;
     unsigned keep = 0;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
@@ -745,17 +770,15 @@ __device__ __forceinline__ bool choose_alone(const RouteParams& p, const T* row,
 #pragma unroll
       for (int i = 0; i < NE; ++i)
         if (i < a.experts && i % size == 0) rank += score[i] > score[j] || (score[i] == score[j] && i / size < j / size) ? 1 : 0;
+      const float v = static_cast<float>(value_of(score[j])), size = static_cast<float>(size_of[j]);
       if (rank < a.top_groups) {
         keep |= 1u << j;
-        low = smaller(low, score[j]);
+        low = fminf(low, least_score(v, size, tau, 0x1p-22f));
       } else {
-        high = larger(high, score[j]);
+        high = fmaxf(high, largest_score(v, size, tau, 0x1p-22f));
       }
     }
-    if (check) {
-      const float a0 = static_cast<float>(value_of(low)), gap = static_cast<float>(value_of(low) - value_of(high));
-      close = !(gap > 2.f * tau + 0x1p-20f * fabsf(a0));
-    }
+    close = check && !(low > high);
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       if (!((keep >> j) & 1u)) key[j] = 0;

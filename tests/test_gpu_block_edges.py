@@ -1,11 +1,12 @@
-"""Routing, dispatch / combine and the block norms on the GPU where they can go wrong: choices that are left out.
-Tolerances as in test_gpu_block_ops.py; what is not rounded is compared bit by bit."""
+"""Routing, dispatch / combine and the block norms on the GPU where they can go wrong: sums that cancel, choices
+that are left out.  Tolerances as in test_gpu_block_ops.py; what is not rounded is compared bit by bit."""
 
 import math
 
 import pytest
 import torch
 
+import block_reference as ref
 from block_reference import HALF_STEP, TINY
 from pccl_b200.ops import Routing, combine, dispatch, route_topk
 
@@ -20,6 +21,26 @@ def _gen(seed):
 
 def _normal(g, *shape):
     return torch.randn(*shape, device="cuda", generator=g)
+
+
+# ------------------------------------------------------------------------------------------------- routing
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [16.0, 512.0, 4096.0])
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [
+    (8, 4, 2, 3), (16, 8, 4, 5), (64, 8, 3, 4), (256, 8, 4, 8), (42, 6, 3, 3), (512, 32, 16, 8), (1000, 20, 7, 9)])
+def test_route_groups_whose_best_two_cancel(experts, groups, top_groups, top_k, size, scoring):
+    """A group's two best biased scores are near +size and -size: their sum has lost what 32 bits of either lose."""
+    g = _gen(experts)
+    each, tokens = experts // groups, 30000 if experts <= 64 else 6000
+    bias = torch.full((groups, each), -2 * size, device="cuda")
+    bias[:, 0], bias[:, 1] = size, -size
+    bias = bias.flatten()
+    logits = 0.7 * _normal(g, tokens, experts)
+    got = route_topk(logits, top_k, bias=bias, scoring=scoring, groups=groups, top_groups=top_groups, group_score="top2")
+    idx, rows, offsets = ref.route(logits, top_k, bias, scoring, groups, top_groups, "top2")
+    wrong = (got.idx.long() != idx).any(-1)
+    assert not bool(wrong.any()), f"{int(wrong.sum())} of {tokens} tokens"
+    assert torch.equal(got.rows.long(), rows) and torch.equal(got.offsets.long(), offsets)
 
 
 # --------------------------------------------------------------------------------------- dispatch / combine
