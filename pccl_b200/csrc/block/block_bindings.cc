@@ -50,6 +50,14 @@ void on_device(const Tensor& t, const Tensor& first, const char* op, const char*
   PCCL_ARG(t.device() == first.device(), op << ": " << what << " must be on the device of the other tensors");
 }
 
+// Tangents of forward-mode differentiation are refused: these operators would lose them without a word.
+void no_tangent(const Tensor& t, const char* op, const char* what) {
+  PCCL_ARG(!t._fw_grad(0).defined(), op << ": " << what << " has a forward-mode tangent, but there are only gradients backwards");
+}
+void no_tangent(const OptTensor& t, const char* op, const char* what) {
+  if (t.has_value()) no_tangent(*t, op, what);
+}
+
 // Rows of `cols` values with unit stride: the tensor itself where it is laid out so, else a copy.
 struct Rows {
   Tensor t;
@@ -215,6 +223,8 @@ variable_list route_topk(const Tensor& logits, int64_t top_k, const OptTensor& b
   }
   if (mask.has_value())
     PCCL_ARG(mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->size(0) == t, op << ": mask must be bool [tokens]");
+  no_tangent(logits, op, "logits");
+  no_tangent(bias, op, "bias");
   on_device(logits, logits, op, "logits");
   if (bias.has_value()) on_device(*bias, logits, op, "bias");
   if (mask.has_value()) on_device(*mask, logits, op, "mask");
@@ -328,6 +338,7 @@ Tensor dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
   const char* op = "dispatch";
   check_move(op, x, rows, offsets);
   PCCL_ARG(x.size(0) == rows.size(0), op << ": x has " << x.size(0) << " rows, the routing " << rows.size(0) << " tokens");
+  no_tangent(x, op, "x");
   on_device(x, x, op, "x");
   on_device(rows, x, op, "routing.rows");
   on_device(offsets, x, op, "routing.offsets");
@@ -341,6 +352,8 @@ Tensor combine(const Tensor& y, const Tensor& weights, const Tensor& rows, const
   PCCL_ARG(y.size(0) == rows.numel(), op << ": y has " << y.size(0) << " rows, the routing " << rows.numel() << " choices");
   PCCL_ARG(weights.scalar_type() == at::kFloat && weights.sizes() == rows.sizes() && weights.is_contiguous(),
            op << ": routing.weights must be contiguous float32 [tokens, top_k]");
+  no_tangent(y, op, "y");
+  no_tangent(weights, op, "routing.weights");
   on_device(y, y, op, "y");
   on_device(weights, y, op, "routing.weights");
   on_device(rows, y, op, "routing.rows");
@@ -530,6 +543,11 @@ std::pair<OptTensor, OptTensor> residual_rms_norm(const Tensor& residual, const 
     c.gate_rows = rows > 0 ? rows / groups : 1;
   }
   PCCL_ARG(eps >= 0, op << ": eps must not be negative");
+  no_tangent(residual, op, first);
+  no_tangent(x, op, "x");
+  no_tangent(gamma, op, "gamma");
+  no_tangent(post_gamma, op, "post_gamma");
+  no_tangent(gate, op, "gate");
   on_device(residual, residual, op, first);
   if (x.has_value()) on_device(*x, residual, op, "x");
   if (gamma.has_value()) on_device(*gamma, residual, op, "gamma");

@@ -1,0 +1,44 @@
+"""Refusals and host paths of routing, dispatch / combine, the block norms and the trainable block that need no GPU."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from pccl_b200.ops import Routing, combine, dispatch, residual_rms_norm, rms_norm, route_topk
+
+
+def _routing(weights=None):
+    return Routing(torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2) if weights is None else weights,
+                   torch.arange(8, dtype=torch.int32).view(4, 2), torch.zeros(9, dtype=torch.int32))
+
+
+CALLS = {
+    "logits": lambda d: route_topk(d(4, 8), 2),
+    "bias": lambda d: route_topk(torch.zeros(4, 8), 2, bias=d(8)),
+    "dispatch: x": lambda d: dispatch(d(4, 16), _routing()),
+    "combine: y": lambda d: combine(d(8, 16), _routing()),
+    "routing.weights": lambda d: combine(torch.zeros(8, 16), _routing(d(4, 2))),
+    "rms_norm: x": lambda d: rms_norm(d(4, 16), torch.zeros(16)),
+    "residual": lambda d: residual_rms_norm(d(4, 16), torch.zeros(4, 16), torch.zeros(16)),
+    "residual_rms_norm: x": lambda d: residual_rms_norm(torch.zeros(4, 16), d(4, 16), torch.zeros(16)),
+    "gamma": lambda d: residual_rms_norm(torch.zeros(4, 16), torch.zeros(4, 16), d(16)),
+    "post_gamma": lambda d: residual_rms_norm(torch.zeros(4, 16), torch.zeros(4, 16), None, post_gamma=d(16)),
+    "gate": lambda d: residual_rms_norm(torch.zeros(4, 16), torch.zeros(4, 16), None, gate=d(2, 16)),
+}
+
+
+@pytest.mark.parametrize("what", CALLS)
+def test_forward_mode_tangents_are_refused(what):
+    """Without this a tensor that carries a tangent, but requires no gradient, would lose it without a word."""
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match=f"{what} has a forward-mode tangent"):
+            CALLS[what](lambda *shape: fwd.make_dual(torch.zeros(shape), torch.ones(shape)))
+        with pytest.raises(ValueError, match="CUDA device"):        # a level alone changes nothing
+            CALLS[what](lambda *shape: torch.zeros(shape))
+
+
+def test_forward_mode_and_requires_grad():
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(4, 16, requires_grad=True), torch.ones(4, 16))
+        with pytest.raises(ValueError, match="forward-mode tangent"):
+            dispatch(x, _routing())
