@@ -102,11 +102,15 @@ class SparseMoEBlock(torch.nn.Module):
         self.w2 = normal(experts, hidden, ffn, scale=ffn ** -0.5)
 
     def experts(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-        """Rows in expert order through their experts; unused rows become zero."""
+        """Rows in expert order through their experts; unused rows become zero.
+
+        Experts without rows are passed over, but for one where none has any: the weights get a gradient, of zero then,
+        in every batch, so that ranks that average them always agree on what there is to reduce.
+        """
         ends = offsets.tolist()
         parts = []
         for e in range(self.w2.shape[0]):
-            if ends[e + 1] > ends[e]:
+            if ends[e + 1] > ends[e] or (e == 0 and ends[-1] == 0):
                 gate, up = (x[ends[e]:ends[e + 1]] @ self.w13[e].t()).chunk(2, dim=-1)
                 parts.append((F.silu(gate) * up) @ self.w2[e].t())
         parts.append(x.new_zeros(x.shape[0] - ends[-1], x.shape[1]))

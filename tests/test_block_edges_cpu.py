@@ -42,3 +42,31 @@ def test_forward_mode_and_requires_grad():
         x = fwd.make_dual(torch.zeros(4, 16, requires_grad=True), torch.ones(4, 16))
         with pytest.raises(ValueError, match="forward-mode tangent"):
             dispatch(x, _routing())
+
+
+@pytest.mark.parametrize("rows", [0, 6])
+def test_experts_without_rows_still_have_gradients(rows):
+    """A batch whose tokens are all masked, or that has none: gradients of zero, not none at all.  With none, ranks that
+    average them would not agree on what there is to reduce."""
+    from pccl_b200.models import SparseMoEBlock
+    block = SparseMoEBlock(16, 32, 4, 2, dtype=torch.float32, device="cpu")
+    x = torch.randn(rows, 16, requires_grad=True)
+    out = block.experts(x, torch.zeros(5, dtype=torch.int32))
+    assert out.shape == (rows, 16) and bool((out == 0).all())
+    out.sum().backward()
+    for t in (block.w13, block.w2, x):
+        assert t.grad is not None and t.grad.shape == t.shape and bool((t.grad == 0).all())
+
+
+def test_experts_on_their_rows():
+    """Some experts without rows, some rows unused, against each row's own products."""
+    from pccl_b200.models import SparseMoEBlock
+    block = SparseMoEBlock(16, 32, 4, 2, dtype=torch.float64, device="cpu")
+    x = torch.randn(7, 16, dtype=torch.float64, requires_grad=True)
+    out = block.experts(x, torch.tensor([0, 2, 2, 5, 5], dtype=torch.int32))
+    for row, e in enumerate((0, 0, 2, 2, 2)):
+        gate, up = (block.w13[e] @ x[row]).chunk(2)
+        torch.testing.assert_close(out[row], block.w2[e] @ (torch.nn.functional.silu(gate) * up))
+    assert bool((out[5:] == 0).all())
+    out.sum().backward()
+    assert bool((block.w13.grad[[1, 3]] == 0).all()) and bool((block.w2.grad[[0, 2]] != 0).any()) and bool((x.grad[5:] == 0).all())

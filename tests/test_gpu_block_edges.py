@@ -145,3 +145,21 @@ def test_moves_captured_with_choices_left_out():
         dead = torch.ones(3000, dtype=torch.bool, device="cuda")
         dead[rows[rows >= 0].long()] = False
         assert bool((outs[0][dead] == 0).all())
+
+
+# ------------------------------------------------------------------------------------- as a user's program has them
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens", [0, 40])
+def test_block_without_live_tokens_has_every_gradient(tokens, dtype):
+    """All tokens masked, and no tokens: every parameter that takes part gets a gradient of the block's type."""
+    from pccl_b200.models import SparseMoEBlock
+    torch.manual_seed(0)
+    block = SparseMoEBlock(64, 96, 8, 2, post_norm=True, gated=True, dtype=dtype)
+    x = torch.randn(tokens, 64, device="cuda").to(dtype).requires_grad_(True)
+    y, stream = block(x, next_gamma=torch.ones(64, dtype=dtype, device="cuda"),
+                      mask=torch.zeros(tokens, dtype=torch.bool, device="cuda"))
+    assert torch.equal(stream, x)                                   # nothing is added to the stream
+    (y.float().square().sum() + stream.float().sum()).backward()
+    for name, p in block.named_parameters():
+        assert p.grad is not None and p.grad.dtype == dtype and bool((p.grad == 0).all()), name
+    assert x.grad.shape == x.shape
