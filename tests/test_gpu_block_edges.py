@@ -163,3 +163,50 @@ def test_block_without_live_tokens_has_every_gradient(tokens, dtype):
     for name, p in block.named_parameters():
         assert p.grad is not None and p.grad.dtype == dtype and bool((p.grad == 0).all()), name
     assert x.grad.shape == x.shape
+
+
+def test_sparse_moe_block_in_its_default_type():
+    """bfloat16, as the class is made by default, against the same operators on its own intermediate values: what the block
+    wires together.  The library products are the same calls, so the results are equal."""
+    from pccl_b200.models import SparseMoEBlock
+    from pccl_b200.ops import residual_rms_norm, rms_norm
+    torch.manual_seed(1)
+    block = SparseMoEBlock(128, 64, 8, 2, post_norm=True, gated=True, balance=True, scoring="sigmoid")
+    assert {p.dtype for p in block.parameters()} == {torch.bfloat16}
+    x = torch.randn(300, 128, device="cuda").bfloat16().requires_grad_(True)
+    gamma = (1 + 0.1 * torch.randn(128, device="cuda")).bfloat16()
+    y, stream = block(x, next_gamma=gamma)
+    grads = torch.autograd.grad(y.float().square().sum() + stream.float().sum(), [x] + list(block.parameters()))
+    n = rms_norm(x, block.gamma)
+    r = route_topk(n.float() @ block.wg.float().t(), 2, bias=block.bias, scoring="sigmoid")
+    rows, ends = dispatch(n, r), r.offsets.tolist()
+    parts = []
+    for e in range(8):
+        gate, up = (rows[ends[e]:ends[e + 1]] @ block.w13[e].t()).chunk(2, dim=-1)
+        parts.append((torch.nn.functional.silu(gate) * up) @ block.w2[e].t())
+    wy, ws = residual_rms_norm(x, combine(torch.cat(parts), r), gamma, post_gamma=block.post_gamma, gate=block.gate)
+    assert torch.equal(y, wy) and torch.equal(stream, ws)
+    wants = torch.autograd.grad(wy.float().square().sum() + ws.float().sum(), [x] + list(block.parameters()))
+    for (name, _), got, want in zip([("x", x)] + list(block.named_parameters()), grads, wants):
+        assert torch.equal(got, want) and got.dtype == torch.bfloat16 and bool((got != 0).any()), name
+
+
+def test_calls_in_inference_mode_and_under_vmap():
+    """Inference mode gives the same results; a batched tensor of vmap is refused, not read as something else."""
+    from pccl_b200.ops import residual_rms_norm
+    g = _gen(6)
+    logits, x, gamma = _normal(g, 50, 16), _normal(g, 50, 64).bfloat16(), torch.ones(64, device="cuda")
+
+    def step():
+        r = route_topk(logits, 2, bias=torch.zeros(16, device="cuda"))
+        return tuple(r) + (out := dispatch(x, r), combine(out, r)) + residual_rms_norm(x, x, gamma)
+
+    want = step()
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(want, step()))
+    r = route_topk(logits, 2)
+    for call in (lambda t: dispatch(t, r), lambda t: residual_rms_norm(t, t, gamma)[0]):
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.vmap(call)(x.expand(3, 50, 64))
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.vmap(lambda t: route_topk(t, 2).weights)(logits.expand(3, 50, 16))
