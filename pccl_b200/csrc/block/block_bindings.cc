@@ -214,7 +214,7 @@ variable_list route_topk(const Tensor& logits, int64_t top_k, const OptTensor& b
            op << ": top_k must be at least 1, at most " << block::kMaxTopK
               << " and at most the experts of the groups that stay");
   PCCL_ARG(!top2 || top_groups == groups || e / groups >= 2, op << ": the sum of a group's two best scores needs groups of two");
-  PCCL_ARG(t * top_k < INT_MAX, op << ": tokens * top_k must stay below 2^31");
+  PCCL_ARG(t * top_k < block::kMaxChoices, op << ": tokens * top_k must stay below 2^31 - 2^16");
   if (bias.has_value()) {
     PCCL_ARG(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == e,
              op << ": bias must be float32 [experts]");

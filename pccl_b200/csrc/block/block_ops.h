@@ -17,6 +17,7 @@ inline int dtype_bytes(DType t) { return t == DType::kF32 ? 4 : 2; }
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 31;     // one lane of a warp per choice, and one for the runner-up
 constexpr int kMaxGroups = 32;
+constexpr int64_t kMaxChoices = (int64_t{1} << 31) - (1 << 16);   // tokens * top_k stay below: a block's tokens more, and it still fits 31 bits
 
 struct RouteArgs {
   const void* logits;         // [tokens] rows of `experts` values, `ld` elements apart

@@ -200,8 +200,10 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
     chosen only where nothing else is left, and then with weight 0.  Plus infinity counts as the largest finite
     logit.  Tokens where ``mask`` (bool ``[tokens]``) is false choose nothing: index and row -1, weight 0.
 
-    Up to 1024 experts, 32 groups and 31 choices.  The four results share one allocation.  ``weights`` carries the gradient of ``logits`` (once: it cannot
-    be differentiated twice); the order of the choices within an expert is that of the tokens, on every run.
+    Up to 1024 experts, 32 groups, 31 choices, and ``tokens * top_k`` below 2^31 - 2^16.  ``weights`` carries the gradient
+    of ``logits`` (once: it cannot be differentiated twice, and there is no forward mode); the order of the choices within
+    an expert is that of the tokens, on every run.  The four results are parts of one allocation, which holds the
+    workspace too: it lives as long as any of them, and ``torch.save`` of one writes all of it (save a ``clone()``).
     """
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"route_topk: scoring must be 'softmax' or 'sigmoid', not {scoring!r}")

@@ -70,3 +70,11 @@ def test_experts_on_their_rows():
     assert bool((out[5:] == 0).all())
     out.sum().backward()
     assert bool((block.w13.grad[[1, 3]] == 0).all()) and bool((block.w2.grad[[0, 2]] != 0).any()) and bool((x.grad[5:] == 0).all())
+
+
+@pytest.mark.parametrize("tokens,text", [(2 ** 31 - 100, "2\\^31"), (2 ** 31 - 2 ** 16, "2\\^31"), (2 ** 31 - 2 ** 16 - 1, "CUDA device"),
+                                         (2 ** 33, "2\\^31")])
+def test_most_tokens_of_a_routing(tokens, text):
+    """Token numbers and a block's tokens on top of them are 31-bit sums in the kernels."""
+    with pytest.raises(ValueError, match=text):
+        route_topk(torch.zeros(1, 1).expand(tokens, 1), 1)
