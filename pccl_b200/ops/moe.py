@@ -173,6 +173,11 @@ class Routing(NamedTuple):
     rows: torch.Tensor      # [tokens, top_k] int32: row of each choice in expert order; -1 for masked tokens
     offsets: torch.Tensor   # [experts + 1] int32
 
+    def __reduce__(self):
+        # Parts of one allocation cannot be written to a file together where their types differ, and each would bring
+        # all of it along.
+        return type(self), tuple(t.clone() for t in self)
+
 
 _block = None
 
@@ -203,7 +208,8 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
     Up to 1024 experts, 32 groups, 31 choices, and ``tokens * top_k`` below 2^31 - 2^16.  ``weights`` carries the gradient
     of ``logits`` (once: it cannot be differentiated twice, and there is no forward mode); the order of the choices within
     an expert is that of the tokens, on every run.  The four results are parts of one allocation, which holds the
-    workspace too: it lives as long as any of them, and ``torch.save`` of one writes all of it (save a ``clone()``).
+    workspace too and lives as long as any of them.  Save the `Routing` itself, or clones of its parts: a part alone
+    would bring the whole allocation along, and torch refuses ``idx`` and ``weights`` of one in the same file.
     """
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"route_topk: scoring must be 'softmax' or 'sigmoid', not {scoring!r}")

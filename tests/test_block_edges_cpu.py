@@ -78,3 +78,16 @@ def test_most_tokens_of_a_routing(tokens, text):
     """Token numbers and a block's tokens on top of them are 31-bit sums in the kernels."""
     with pytest.raises(ValueError, match=text):
         route_topk(torch.zeros(1, 1).expand(tokens, 1), 1)
+
+
+def test_a_routing_of_one_allocation_is_pickled():
+    """Its parts as route_topk makes them: whole numbers and weights in one storage, which torch.save refuses to write."""
+    import copy
+    import io
+    all_ = torch.arange(100, dtype=torch.int32)
+    r = Routing(all_[:8].view(4, 2), all_.view(torch.float32)[8:16].view(4, 2), all_[16:24].view(4, 2), all_[24:33])
+    file = io.BytesIO()
+    torch.save({"layer": r}, file)
+    file.seek(0)
+    for copied in (torch.load(file, weights_only=False)["layer"], copy.deepcopy(r), r._replace(rows=r.rows)):
+        assert type(copied) is Routing and all(torch.equal(a, b) for a, b in zip(copied, r))

@@ -1,6 +1,8 @@
 """Routing, dispatch / combine and the block norms on the GPU where they can go wrong: sums that cancel, choices
 that are left out.  Tolerances as in test_gpu_block_ops.py; what is not rounded is compared bit by bit."""
 
+import copy
+import io
 import math
 
 import pytest
@@ -148,6 +150,19 @@ def test_moves_captured_with_choices_left_out():
 
 
 # ------------------------------------------------------------------------------------- as a user's program has them
+@pytest.mark.parametrize("tokens", [1, 5000])
+def test_a_routing_is_saved_and_copied(tokens):
+    """All of a routing in one file, as a program does that replays one, with no more bytes than it has; and a deep copy."""
+    r = route_topk(_normal(_gen(7), tokens, 64), 4)
+    file = io.BytesIO()
+    torch.save(r, file)
+    assert len(file.getvalue()) < tokens * 4 * 12 + 65 * 4 + 16384
+    file.seek(0)
+    for copied in (torch.load(file, weights_only=False), copy.deepcopy(r)):
+        assert type(copied) is Routing
+        assert all(torch.equal(a, b) and a.dtype == b.dtype and a.data_ptr() != b.data_ptr() for a, b in zip(copied, r))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("tokens", [0, 40])
 def test_block_without_live_tokens_has_every_gradient(tokens, dtype):
