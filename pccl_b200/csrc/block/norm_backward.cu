@@ -20,10 +20,10 @@ namespace block {
 namespace norm {
 namespace {
 
-// Slots of a thread, in bytes: gamma, g1 (kFull: a norm behind the block or a gate), its share of the ring.  x is read where h is formed again (16-bit streams) or its norm is undone.
+// Slots of a thread, in bytes: gamma (the first), g1 (kFull: a norm behind the block or a gate), its share of the ring.  x is read where h is formed again (16-bit streams) or its norm is undone.
 template <typename TX, typename TR, bool kFull> struct BackwardSlots {
   static constexpr bool kReadsX = kFull || sizeof(TR) == 2;
-  static constexpr int kGamma = 0, kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
+  static constexpr int kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
   static constexpr int kDy = kBytes<TR>, kH = kDy + kBytes<TX>, kX = kH + kBytes<TR>;
   static constexpr int kShare = kX + (kReadsX ? kBytes<TX> : 0);
   static constexpr int kWindows = kReadsX ? 4 : 3;
@@ -362,10 +362,14 @@ template <typename TX, typename TR, bool kFull>
 void backward_mode(NormParams& p, bool vec, cudaStream_t stream) {
   const Layout l = backward_layout<TX, TR, kFull>(p.a, vec, &p.workers);
   p.ring = l.ring;
-  if (vec && l.split > 1) launch(norm_backward_kernel<TX, TR, kRing, kFull, true>, p, l, stream);
-  else if (vec) launch(norm_backward_kernel<TX, TR, kRing, kFull, false>, p, l, stream);
-  else if (l.split > 1) launch(norm_backward_kernel<TX, TR, kWindow, kFull, true>, p, l, stream);
-  else launch(norm_backward_kernel<TX, TR, kWindow, kFull, false>, p, l, stream);
+  const auto go = [&](auto kernel) {
+    allow_smem(kernel, l);
+    launch(kernel, p, l, stream);
+  };
+  if (vec && l.split > 1) go(norm_backward_kernel<TX, TR, kRing, kFull, true>);
+  else if (vec) go(norm_backward_kernel<TX, TR, kRing, kFull, false>);
+  else if (l.split > 1) go(norm_backward_kernel<TX, TR, kWindow, kFull, true>);
+  else go(norm_backward_kernel<TX, TR, kWindow, kFull, false>);
 }
 
 // Calls f(TX(), TR(), kFull) for the types and weights of these arguments.

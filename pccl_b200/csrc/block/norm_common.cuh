@@ -306,7 +306,7 @@ constexpr int kMostRing = 4;
 // How a row of `hidden` columns is laid out over blocks.  weights and share are bytes a thread, of its weights and of
 // its share of a row; windows is how many windows a row has beyond those bytes.
 struct Layout {
-  int mode, split, threads, ring;
+  int split, threads, ring;
   size_t smem;
 };
 // Registers let 512 threads of 128 registers (or 1024 of 64) share an SM.
@@ -317,7 +317,7 @@ inline int blocks_per_sm(int threads) { return threads < 512 ? 512 / threads : 1
 inline Layout layout_of(int hidden, bool vec, int weights, int share, int windows, int most_threads, bool alone) {
   Layout l{};
   const auto fits = [&](int split, int least) {
-    l = Layout{vec ? kRing : kWindow, split, threads_of(hidden, split), 0, 0};
+    l = Layout{split, threads_of(hidden, split), 0, 0};
     if (l.threads > most_threads) return false;
     const auto bytes = [&](int rows) {
       return static_cast<size_t>(weights + rows * share) * l.threads + (vec ? 0 : static_cast<size_t>(rows) * windows * 16);
@@ -333,9 +333,12 @@ inline Layout layout_of(int hidden, bool vec, int weights, int share, int window
   return l;
 }
 
-template <class Kernel> void launch(Kernel kernel, const NormParams& p, const Layout& l, cudaStream_t stream) {
+// Before a launch, and before a question for its occupancy.
+template <class Kernel> void allow_smem(Kernel kernel, const Layout& l) {
   if (l.smem > 40 * 1024)
     PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.smem)));
+}
+template <class Kernel> void launch(Kernel kernel, const NormParams& p, const Layout& l, cudaStream_t stream) {
   if (l.split == 1) {
     kernel<<<p.workers, l.threads, l.smem, stream>>>(p);
     return;

@@ -15,9 +15,9 @@ namespace block {
 namespace norm {
 namespace {
 
-// Slots of a thread, in bytes: gamma, g1 (kFull: a norm behind the block or a gate), its share of the ring.
+// Slots of a thread, in bytes: gamma (the first), g1 (kFull: a norm behind the block or a gate), its share of the ring.
 template <typename TX, typename TR, bool kFull> struct ForwardSlots {
-  static constexpr int kGamma = 0, kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
+  static constexpr int kG1 = kBytes<float>, kWeights = kBytes<float> * (kFull ? 2 : 1);
   static constexpr int kX = kBytes<TR>, kShare = kBytes<TR> + kBytes<TX>;
 };
 
@@ -150,8 +150,7 @@ template <typename TX, typename TR, int kMode, bool kFull, bool kSplit, int kMos
 void forward_launch(NormParams& p, const Layout& l, cudaStream_t stream) {
   // One wave of blocks: a block's later rows are on their way while it works.
   const auto kernel = norm_forward_kernel<TX, TR, kMode, kFull, kSplit, kMost>;
-  if (l.smem > 40 * 1024)
-    PCCL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(l.smem)));
+  allow_smem(kernel, l);
   const int64_t most = static_cast<int64_t>(max_coresident(kernel, l.threads, l.smem)) / l.split;
   PCCL_CHECK(most > 0, "block norm: the kernel does not fit on this device");
   p.workers = static_cast<int>(p.a.rows < most ? p.a.rows : most);

@@ -1,4 +1,5 @@
-// Loads and stores of eight values between memory of any of the three types and 32-bit registers.
+// Values of the three types and 32-bit registers: conversions one and two at a time, packed 32-bit arithmetic, sums over a
+// warp.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,20 +22,7 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive values, as they lie in memory: 16 bytes of a 16-bit type, 32 of a 32-bit one.
-template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
-
-template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
-  return r;
-}
-template <typename T> __device__ __forceinline__ void store_raw8(T* p, const Raw8<T>& r) {
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
-}
-
+// Two neighbours, as they lie in a 32-bit word.
 __device__ __forceinline__ void unpack2(uint32_t w, float* f, __nv_bfloat16) {
   f[0] = __uint_as_float(w << 16);
   f[1] = __uint_as_float(w & 0xffff0000u);
@@ -51,35 +39,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-template <typename T> __device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f[4 * i] = __uint_as_float(r.v[i].x);
-      f[4 * i + 1] = __uint_as_float(r.v[i].y);
-      f[4 * i + 2] = __uint_as_float(r.v[i].z);
-      f[4 * i + 3] = __uint_as_float(r.v[i].w);
-    }
-  } else {
-    unpack2(r.v[0].x, f, T());
-    unpack2(r.v[0].y, f + 2, T());
-    unpack2(r.v[0].z, f + 4, T());
-    unpack2(r.v[0].w, f + 6, T());
-  }
-}
-template <typename T> __device__ __forceinline__ Raw8<T> pack8(const float* f) {
-  Raw8<T> r;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      r.v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
-                          __float_as_uint(f[4 * i + 3]));
-  } else {
-    r.v[0] = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
-  }
-  return r;
 }
 
 // Two 32-bit operations an instruction (sm_100), each rounded like its scalar form.
