@@ -531,6 +531,7 @@ std::pair<OptTensor, OptTensor> residual_rms_norm(const Tensor& residual, const 
     PCCL_ARG(residual.scalar_type() == xt || residual.scalar_type() == at::kFloat,
              op << ": residual must have the type of x or float32");
   }
+  PCCL_ARG(x.has_value() || gamma.has_value(), op << ": gamma is missing");
   check_weight(op, gamma, hidden, xt, "gamma");
   check_weight(op, post_gamma, hidden, xt, "post_gamma");
   NormCall c{scale, eps, 1};

@@ -91,3 +91,10 @@ def test_a_routing_of_one_allocation_is_pickled():
     file.seek(0)
     for copied in (torch.load(file, weights_only=False)["layer"], copy.deepcopy(r), r._replace(rows=r.rows)):
         assert type(copied) is Routing and all(torch.equal(a, b) for a, b in zip(copied, r))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_rms_norm_needs_its_gamma(grad):
+    """It returned None."""
+    with pytest.raises(ValueError, match="rms_norm: gamma"):
+        rms_norm(torch.zeros(4, 16, requires_grad=grad), None)
