@@ -99,12 +99,13 @@ __device__ __forceinline__ float quick_sigmoid(float l) {
   return r;
 }
 
-// Bound of the difference of two scores' errors; quick_exp(x) is off by (2 + 1.2 |x|) 2^-23 of itself.  Sigmoid:
-// p (1 - p) times that is at most 0.7 * 2^-23, the sum adds 2^-24 and the reciprocal 2^-23: 1.1 * 2^-21 for two.  Softmax: of the row's largest
-// probability, exponential 5 * 2^-24 (|x| e^-|x| < 0.37), the sum over a lane and the warp (n + 5) 2^-24 and its terms'
-// 5 * 2^-24, quotient and product 3 * 2^-24.
+// Bound of the difference of two scores' errors; quick_exp(x) is off by (2 + 0.63 |x|) 2^-23 of itself (the instruction's
+// 2^-22, the product's rounding and the constant's).  Sigmoid: p (1 - p) times that is at most 0.52 * 2^-23, the sum adds
+// p 2^-24 and the reciprocal p 2^-23: below 1.7 * 2^-23 for one, 2^-21 for two.  Softmax: of the row's largest probability,
+// the exponential 4 * 2^-24 ((2 + 0.63 |x|) e^-|x| is largest at 0), the sum over a lane and the warp (n + 5) 2^-24 and its
+// terms' own 10 * 2^-24 (1023 terms at |x| = 5.5 beside one at 0 are the worst), quotient and product 3 * 2^-24.
 __device__ __forceinline__ float score_error(bool sigmoid_scores, int n, float largest) {
-  return sigmoid_scores ? 0x1.4p-21f : static_cast<float>(n + 20) * 0x1p-23f * largest;
+  return sigmoid_scores ? 0x1.4p-21f : static_cast<float>(n + 24) * 0x1p-23f * largest;
 }
 
 // ---- a warp per token ------------------------------------------------------------------------------------------
